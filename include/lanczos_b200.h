@@ -307,7 +307,7 @@ int lg_cgs2_orthogonalize_noalloc(const double* V, int ldv, int n, int ncols, co
  * lg_slq_small_side / lg_slq_block_* calls alone).  Calls sharing a workspace
  * must be ordered on one stream.
  */
-enum { LG_F32 = 0, LG_F64 = 1 };
+enum { LG_F32 = 0, LG_F64 = 1, LG_F16 = 2, LG_BF16 = 3 };   /* the 16-bit types: node features only */
 enum { LG_FUNC_LOG = 0, LG_FUNC_EXP = 1, LG_FUNC_SQRT = 2, LG_FUNC_INV = 3 };
 
 /* P = A^power with A = shift I + L; L symmetric, given as its diagonal and its
@@ -481,6 +481,76 @@ int lg_knn_laplacian_fill(int n, int k, const long long* idx, const double* d2, 
  * operations of funm_apply_kraemer (python/gpu_eigsh/funm_torch.py:284, 347). */
 int lg_dense_matvec(int n, int dtype, const void* A, const void* x, int ldx, void* y, int ldy, void* stream);
 int lg_outer_accumulate(int n, int dtype, const void* lam, const void* x, int ld, double* gA, void* stream);
+
+/* ---- node features ------------------------------------------------------ */
+/* Row-major feature rows of `dim` values of one element type (LG_F32, LG_F64,
+ * LG_F16, LG_BF16) on the device, with row strides ld_* >= dim in elements;
+ * outputs are contiguous.  Arithmetic, sums and the parameters said to be in
+ * the accumulation type are in fp64 for LG_F64, else in fp32; results are
+ * rounded once.  Every call only enqueues work on `stream`; sums run in a fixed
+ * order, so equal inputs give equal bits.  Addresses and strides may have any
+ * alignment; multiples of 16 bytes are fastest. */
+
+/* out[t, :] = s * table[ids[t], :] for t < n (ids: int64, or int32 when ids64 =
+ * 0).  scale_mode LG_SCALE_NONE, LG_SCALE_VALUE (s = scale_value) or
+ * LG_SCALE_COLUMN (scale: dim values of the accumulation type).  With
+ * has_padding an id equal to `padding` (any integer) gives a row of zeros; any
+ * other id outside [0, rows) reads nothing and gives a row of NaN. */
+#define LG_SCALE_NONE 0
+#define LG_SCALE_VALUE 1
+#define LG_SCALE_COLUMN 2
+int lg_rows_gather(long long rows, int dim, int dtype, const void* table, long long ld_table, long long n,
+                   const void* ids, int ids64, int scale_mode, const void* scale, double scale_value, int has_padding,
+                   long long padding, void* out, void* stream);
+
+/* The gradient of lg_rows_gather for g = dL/d out (n x dim): d_table (rows x
+ * dim, written whole: zero rows where no id points) and, for LG_SCALE_COLUMN,
+ * d_scale (dim values of the accumulation type; needs `table`).  Either may be
+ * NULL.  Padding and out-of-range ids contribute nothing.  The rows of one id
+ * are added in the order of t. */
+size_t lg_rows_scatter_workspace_bytes(long long rows, int dim, int dtype, long long n, int want_scale);
+int lg_rows_scatter(long long rows, int dim, int dtype, const void* table, long long ld_table, long long n,
+                    const void* ids, int ids64, int scale_mode, const void* scale, double scale_value, int has_padding,
+                    long long padding, const void* g, long long ld_g, void* d_table, void* d_scale, void* ws,
+                    size_t ws_bytes, void* stream);
+
+/* y = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) * weight + bias, row by
+ * row.  weight and bias (either may be NULL) are of param_dtype: the element
+ * type, or LG_F32 for the 16-bit types.  mean and rstd (rows values of the
+ * accumulation type; both or neither NULL) keep the rows' statistics for the
+ * backward pass, which gives dx, d_weight and d_bias (any may be NULL). */
+int lg_layer_norm_forward(long long rows, int dim, int dtype, const void* x, long long ld_x, int param_dtype,
+                          const void* weight, const void* bias, double eps, void* y, void* mean, void* rstd,
+                          void* stream);
+size_t lg_layer_norm_workspace_bytes(long long rows, int dim, int dtype, int want_weight, int want_bias);
+int lg_layer_norm_backward(long long rows, int dim, int dtype, const void* x, long long ld_x, const void* g,
+                           long long ld_g, int param_dtype, const void* weight, const void* mean, const void* rstd,
+                           void* dx, void* d_weight, void* d_bias, void* ws, size_t ws_bytes, void* stream);
+
+/* The edges of a graph of n vertices, prepared for the two calls below: idx
+ * (device, 2 x m int64: begins, then ends) gives ends (2m: the same, int32) and
+ * for every vertex the list of its edges (rowptr n + 1; other: the vertex at
+ * the other end; eid: the edge), the edges it begins before those it ends,
+ * ascending.  *bad (device int) becomes 1 if an index is outside [0, n); the
+ * lists are then not to be used.  2m < 2^31 - 1. */
+#define LG_EDGE_CHUNK 256
+size_t lg_edge_graph_workspace_bytes(long long n, long long m);
+int lg_edge_graph(long long n, long long m, const long long* idx, int* ends, int* rowptr, int* other, int* eid,
+                  int* bad, void* ws, size_t ws_bytes, void* stream);
+/* d2[e] = |x[begin_e, :] - x[end_e, :]|^2 in the accumulation type: the
+ * x_edge_dists of the IMGP operator. */
+int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x, long long ld_x,
+                   void* d2, void* stream);
+/* dx[v, :] = 2 sum over the edges e at v of g[e] (x[v, :] - x[other end, :]),
+ * g = dL/d d2.  The vertices with more than LG_EDGE_CHUNK edges are listed by
+ * the caller: long_row (nlong vertices), long_first (index of each one's first
+ * chunk), and for each of the nchunks pieces of LG_EDGE_CHUNK list entries
+ * (vertex by vertex) chunk_row and chunk_first (its first position in eid). */
+size_t lg_edge_sqdist_grad_workspace_bytes(int nchunks, int dim, int dtype);
+int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype, const int* rowptr, const int* other,
+                        const int* eid, int nlong, const int* long_row, const int* long_first, int nchunks,
+                        const int* chunk_row, const int* chunk_first, const void* x, long long ld_x, const void* g,
+                        void* dx, void* ws, size_t ws_bytes, void* stream);
 
 const char* lg_status_string(int status);
 /* Copies the last error message of the calling thread; returns its length. */

@@ -85,6 +85,10 @@ class EigshInfo(C.Structure):
 
 LG_F32 = 0
 LG_F64 = 1
+LG_F16 = 2
+LG_BF16 = 3
+LG_SCALE_NONE, LG_SCALE_VALUE, LG_SCALE_COLUMN = 0, 1, 2
+LG_EDGE_CHUNK = 256
 FUNCS = {"log": 0, "exp": 1, "sqrt": 2, "inv": 3}
 
 
@@ -110,6 +114,7 @@ _PI = C.POINTER(C.c_int)
 _V = C.c_void_p
 _I = C.c_int
 _SZ = C.c_size_t
+_L = C.c_longlong
 _POP = C.POINTER(SlqOp)
 
 # Every exported symbol with its ctypes signature (restype, argtypes).
@@ -168,6 +173,17 @@ SIGNATURES = {
     "lg_knn_laplacian_fill": (_I, [_I, _I, _V, _V, C.c_double, _V, _V, _V, _V]),
     "lg_dense_matvec": (_I, [_I, _I, _V, _V, _I, _V, _I, _V]),
     "lg_outer_accumulate": (_I, [_I, _I, _V, _V, _I, _V, _V]),
+    "lg_rows_gather": (_I, [_L, _I, _I, _V, _L, _L, _V, _I, _I, _V, C.c_double, _I, _L, _V, _V]),
+    "lg_rows_scatter_workspace_bytes": (_SZ, [_L, _I, _I, _L, _I]),
+    "lg_rows_scatter": (_I, [_L, _I, _I, _V, _L, _L, _V, _I, _I, _V, C.c_double, _I, _L, _V, _L, _V, _V, _V, _SZ, _V]),
+    "lg_layer_norm_forward": (_I, [_L, _I, _I, _V, _L, _I, _V, _V, C.c_double, _V, _V, _V, _V]),
+    "lg_layer_norm_workspace_bytes": (_SZ, [_L, _I, _I, _I, _I]),
+    "lg_layer_norm_backward": (_I, [_L, _I, _I, _V, _L, _V, _L, _I, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),
+    "lg_edge_graph_workspace_bytes": (_SZ, [_L, _L]),
+    "lg_edge_graph": (_I, [_L, _L, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),
+    "lg_edge_sqdist": (_I, [_L, _L, _I, _I, _V, _V, _L, _V, _V]),
+    "lg_edge_sqdist_grad_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "lg_edge_sqdist_grad": (_I, [_L, _L, _I, _I, _V, _V, _V, _I, _V, _V, _I, _V, _V, _V, _L, _V, _V, _V, _SZ, _V]),
     "lg_eigsh_adjoint": (_I, [_I, C.c_longlong, _V, _V, _V, _I, _V, _V, _V, _V, _V, _I, C.c_double, _PI, _V]),
     "compute_adjoint_eigsh": (_I, [_I, _I, _PI, _PI, _PD, _I, _PD, _PD, _PD, _PD, _PD, _I, C.c_double]),
     "lg_eigsh_plan_funm": (_I, [_V, _V, _I, _I, _I, _I, _V, _PD, _PI]),
