@@ -27,6 +27,7 @@ import numpy as np
 import torch
 
 from . import _native
+from .features import layer_norm
 
 __all__ = ["knn", "knn_laplacian", "generate_points", "generate_knn_laplacian"]
 
@@ -44,15 +45,27 @@ def _device_points(points) -> torch.Tensor:
     return points.to(dev, torch.float64).contiguous()
 
 
-def knn(points, k: int, method: str = "auto"):
+def _normalized(points) -> torch.Tensor:
+    """Every point with mean 0 and variance 1 over its coordinates
+    (gpu_eigsh.features.layer_norm in fp64)."""
+    P = _device_points(points)
+    if P.shape[1] < 2:
+        raise ValueError("normalize needs points of at least two coordinates")
+    return layer_norm(P, eps=1e-12)
+
+
+def knn(points, k: int, method: str = "auto", normalize: bool = False):
     """Exact k nearest neighbours (self excluded) of the rows of `points`
     ((n, dim), host array or tensor; computed on the GPU).  Returns device
     tensors (idx (n, k) int64, d2 (n, k) float64), each row ascending by
     (squared distance, index).  method: "auto" (cell grid for dim <= 3,
-    else all pairs), "cells" or "brute"."""
+    else all pairs), "cells" or "brute".
+
+    normalize: layer-normalise every point first, so that neighbours are by
+    correlation: d2 = 2 dim (1 - correlation of the two points' coordinates)."""
     if method not in _native.KNN_METHODS:
         raise ValueError(f"method must be one of {sorted(_native.KNN_METHODS)}")
-    P = _device_points(points)
+    P = _normalized(points) if normalize else _device_points(points)
     n, dim = P.shape
     k = int(k)
     if not 1 <= k < n:
@@ -86,10 +99,10 @@ def laplacian_from_knn(idx: torch.Tensor, d2: torch.Tensor, bw: float):
     return rowptr, col, val
 
 
-def knn_laplacian(points, k: int, bw: float, method: str = "auto"):
+def knn_laplacian(points, k: int, bw: float, method: str = "auto", normalize: bool = False):
     """The kNN graph Laplacian of the reference's builders, on the GPU:
-    device (rowptr, col, val); see laplacian_from_knn."""
-    idx, d2 = knn(points, k, method)
+    device (rowptr, col, val); see laplacian_from_knn and, for normalize, knn."""
+    idx, d2 = knn(points, k, method, normalize)
     return laplacian_from_knn(idx, d2, bw)
 
 
@@ -100,12 +113,12 @@ def generate_points(n: int, dim: int, seed: int) -> np.ndarray:
 
 
 def generate_knn_laplacian(n: int = 100000, dim: int = 10, k: int = 15, bw: float = 0.3, seed: int = 123,
-                           method: str = "auto"):
+                           method: str = "auto", normalize: bool = False):
     """The matrix of benchmark/generate_large_laplacian.py (same defaults),
     built on the GPU.  Returns a scipy CSR (float64)."""
     import scipy.sparse as sp
 
-    rp, col, val = knn_laplacian(generate_points(n, dim, seed), k, bw, method)
+    rp, col, val = knn_laplacian(generate_points(n, dim, seed), k, bw, method, normalize)
     return sp.csr_matrix((val.cpu().numpy(), col.cpu().numpy(), rp.cpu().numpy()), shape=(n, n))
 
 
@@ -118,12 +131,14 @@ def main(argv=None) -> int:
     ap.add_argument("--bw", type=float, default=0.3)
     ap.add_argument("--seed", type=int, default=123)
     ap.add_argument("--method", default="auto", choices=sorted(_native.KNN_METHODS))
+    ap.add_argument("--normalize", action="store_true",
+                    help="layer-normalise the points first: neighbours by correlation")
     ap.add_argument("--outdir", default="data")
     a = ap.parse_args(argv)
     from .io import mmwrite
 
     t0 = time.perf_counter()
-    L = generate_knn_laplacian(a.n, a.dim, a.k, a.bw, a.seed, a.method)
+    L = generate_knn_laplacian(a.n, a.dim, a.k, a.bw, a.seed, a.method, a.normalize)
     t1 = time.perf_counter()
     os.makedirs(a.outdir, exist_ok=True)
     out = os.path.join(a.outdir, "laplacian.mtx")

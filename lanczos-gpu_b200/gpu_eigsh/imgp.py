@@ -35,6 +35,7 @@ import math
 import torch
 
 from . import _native, _slq
+from .features import embedding_lookup
 
 __all__ = ["make_imgp_precision_matvec", "ImgpPrecisionMatvec", "_matmul_symmetric_laplacian",
            "imgp_neg_marginal_log_likelihood"]
@@ -44,6 +45,11 @@ _MAXB = 128
 
 def _scalar(t) -> float:
     return float(t.detach().reshape(-1)[0]) if torch.is_tensor(t) else float(t)
+
+
+def _rows(X: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
+    """X[at] for an (n, B) block: the library's row lookup."""
+    return embedding_lookup(X, at) if X.dim() == 2 and X.numel() else X.index_select(0, at)
 
 
 class ImgpPrecisionMatvec:
@@ -109,10 +115,10 @@ class ImgpPrecisionMatvec:
 
     def to_internal(self, X: torch.Tensor) -> torch.Tensor:
         """Rows of X (caller's vertex order) in the operator's row order."""
-        return X if self.perm is None else X.index_select(0, self.perm)
+        return X if self.perm is None else _rows(X, self.perm)
 
     def to_caller(self, Y: torch.Tensor) -> torch.Tensor:
-        return Y if self.pos is None else Y.index_select(0, self.pos)
+        return Y if self.pos is None else _rows(Y, self.pos)
 
     # -- L_sym(kappa) and dL/dkappa -----------------------------------------------
     def laplacian(self, kappa: float):

@@ -700,6 +700,27 @@ def test_features_to_eigenvalues_to_features():
         assert float(t.abs().max()) <= 1e-7 * float(gr[1].abs().max())
 
 
+def test_knn_of_normalised_points():
+    """graph.knn(normalize=True) is knn of the layer-normalised points; its squared distances are
+    2 dim (1 - correlation) of the points' coordinates."""
+    from gpu_eigsh.features import layer_norm
+    from gpu_eigsh.graph import knn, knn_laplacian
+
+    P = randn((400, 10), F64, 1, 3.0, 5.0)
+    idx, d2 = knn(P, 7, normalize=True)
+    ref_i, ref_d = knn(layer_norm(P, eps=1e-12), 7)
+    assert torch.equal(idx, ref_i) and torch.equal(d2, ref_d)
+    corr = torch.corrcoef(P)
+    # eps moves the variance by 1e-12 of itself (variances here are of order 9)
+    want = 20.0 * (1.0 - torch.gather(corr, 1, idx))
+    assert float((d2 - want).abs().max()) < 1e-11
+    rp, col, val = knn_laplacian(P, 7, 0.5, normalize=True)
+    rp2, col2, val2 = knn_laplacian(layer_norm(P, eps=1e-12), 7, 0.5)
+    assert torch.equal(rp, rp2) and torch.equal(col, col2) and torch.equal(val, val2)
+    with pytest.raises(ValueError):
+        knn(P[:, :1], 3, normalize=True)
+
+
 def test_distances_drive_the_graph_gp():
     """The distances as x_edge_dists of the IMGP operator, and their gradient through slq_logdet of a torch matvec."""
     from gpu_eigsh.features import EdgeDistances, layer_norm
