@@ -177,7 +177,7 @@ SIGNATURES = {
     "lg_rows_scatter_workspace_bytes": (_SZ, [_L, _I, _I, _L, _I]),
     "lg_rows_scatter": (_I, [_L, _I, _I, _V, _L, _L, _V, _I, _I, _V, C.c_double, _I, _L, _V, _L, _V, _V, _V, _SZ, _V]),
     "lg_layer_norm_forward": (_I, [_L, _I, _I, _V, _L, _I, _V, _V, C.c_double, _V, _V, _V, _V]),
-    "lg_layer_norm_workspace_bytes": (_SZ, [_L, _I, _I, _I, _I]),
+    "lg_layer_norm_workspace_bytes": (_SZ, [_L, _I, _I]),
     "lg_layer_norm_backward": (_I, [_L, _I, _I, _V, _L, _V, _L, _I, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),
     "lg_edge_graph_workspace_bytes": (_SZ, [_L, _L]),
     "lg_edge_graph": (_I, [_L, _L, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),

@@ -253,7 +253,7 @@ class _LayerNorm(torch.autograd.Function):
             g2, ld_g = _rows2d(g, dim)
             nb, ws = 0, None
             if need_w or need_b:
-                nb = _L.lg_layer_norm_workspace_bytes(rows, dim, code, need_w, need_b)
+                nb = _L.lg_layer_norm_workspace_bytes(rows, dim, code)
                 ws = torch.empty(nb, dtype=torch.uint8, device=dev)
             _call(dev, _L.lg_layer_norm_backward, rows, dim, code, x2.data_ptr(), ld_x, g2.data_ptr(), ld_g,
                   _CODES[pdtype], _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
