@@ -16,16 +16,21 @@
 // pieces of a row (long rows) in flight before the first store.  Bound by
 // memory: nothing is reused but rows named twice.
 //
-// Gradient: the ids are sorted (stable, with their positions), the sorted
-// positions are cut into tiles of equal length, and a group of lanes sums the
-// rows of one tile, one vector of columns per lane.  Equal tiles keep the work
-// even whatever the distribution of the ids.  A run of equal ids inside a tile
-// is finished and written at once; one that crosses a tile's border leaves
-// partial sums (Acc<T>) that the join kernel adds in tile order.  No atomics:
-// the result does not change from run to run.
+// Gradient: the ids are sorted (stable, with their positions) and the sorted
+// positions cut into tiles of equal length; a group of lanes sums the rows of one
+// tile, one vector of columns per lane.  Equal tiles keep the work even whatever
+// the distribution of the ids.  A run of equal ids inside a tile is finished and
+// written at once.  One that crosses tiles leaves partial sums (Acc<T>): in shared
+// memory for the tiles of one block, which are added up there, and in memory for
+// runs that cross blocks, which the last of their blocks to finish adds up in
+// block order.  No sum depends on which block that is, so the result does not
+// change from run to run.  Rows that no id names are set to zero by further blocks
+// of the same launch.
 #include "lg_feat.cuh"
 
 #include "../../include/lanczos_b200.h"
+
+#include <cooperative_groups.h>
 
 namespace lg {
 namespace feat {
@@ -273,6 +278,123 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same sort in one launch, by one cluster: up to kClusterMost ids in 8
+// blocks, up to kBlockMost in one.  The blocks exchange their digit counts
+// through distributed shared memory and the pairs through L2; a cluster barrier
+// stands where the other form has a launch.  Digits of up to 10 bits, so two
+// passes for up to 2^20 rows.  Every thread keeps its ITEMS pairs and their places
+// among the equal digits of its warp from the counting on.
+// ---------------------------------------------------------------------------
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterCtas = 8;
+constexpr int kBlockMost = 4 * kClusterThreads;
+constexpr int kClusterMost = 16 * kClusterThreads * kClusterCtas;
+
+struct ClusterSortArgs {
+  SortArgs s;              // n, rows, ids; in / out as below
+  uint2* buf[2];
+  int passes, width;
+  unsigned* zero;          // words to clear for the kernels that follow
+  int nzero;
+};
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(ClusterSortArgs c) {
+  extern __shared__ unsigned smem[];
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+  const int digits = 1 << c.width, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned* own = smem + (size_t)warp * digits;                  // counts of this warp, then its places
+  unsigned* all = smem + (size_t)kClusterWarps * digits;         // [block][digit] counts
+  __shared__ unsigned scratch[kClusterWarps];
+  for (int i = me * kClusterThreads + threadIdx.x; i < c.nzero; i += ctas * kClusterThreads) c.zero[i] = 0;
+  const long long p0 = ((long long)(me * kClusterWarps + warp) * ITEMS) * 32 + lane;
+  cluster.sync();   // every block runs before its shared memory is written
+  for (int pass = 0; pass < c.passes; ++pass) {
+    SortArgs a = c.s;
+    a.in = pass ? c.buf[(pass - 1) & 1] : nullptr;
+    const int shift = pass * c.width, mask = digits - 1;
+    uint2 kv[ITEMS];
+    unsigned place[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const long long p = p0 + 32 * i;
+      kv[i] = make_uint2(0, 0);
+      if (p < a.n) kv[i] = pass ? __ldcg(a.in + p) : sort_pair(a, p);
+    }
+    for (int i = threadIdx.x; i < kClusterWarps * digits; i += kClusterThreads) smem[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const unsigned act = __ballot_sync(0xffffffffu, p0 + 32 * i < a.n);
+      if (p0 + 32 * i < a.n) {
+        const unsigned d = (kv[i].x >> shift) & mask;
+        const unsigned peers = __match_any_sync(act, d);
+        const unsigned rank = __popc(peers & ((1u << lane) - 1));
+        const unsigned at = own[d];
+        __syncwarp(act);
+        if (rank == 0) own[d] = at + __popc(peers);
+        __syncwarp(act);
+        place[i] = at + rank;
+      }
+    }
+    __syncthreads();
+    const int d = threadIdx.x;
+    unsigned total = 0;
+    if (d < digits) {
+      for (int w = 0; w < kClusterWarps; ++w) total += smem[w * digits + d];
+      for (int q = 0; q < ctas; ++q) cluster.map_shared_rank(all, q)[me * digits + d] = total;
+    }
+    cluster.sync();
+    unsigned below = 0;
+    total = 0;
+    if (d < digits) {
+      for (int q = 0; q < ctas; ++q) {
+        const unsigned v = all[q * digits + d];
+        if (q < me) below += v;
+        total += v;
+      }
+    }
+    unsigned base = digit_prefix(total, scratch) + below;
+    if (d < digits) {
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const unsigned v = smem[w * digits + d];
+        smem[w * digits + d] = base;
+        base += v;
+      }
+    }
+    __syncthreads();
+    uint2* out = c.buf[pass & 1];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (p0 + 32 * i < a.n) out[own[(kv[i].x >> shift) & mask] + place[i]] = kv[i];
+    cluster.sync();   // the pairs are in memory, and `all` may be written again
+  }
+}
+
+template <int ITEMS> cudaError_t launch_cluster_sort(const ClusterSortArgs& c, int ctas, cudaStream_t st) {
+  const int smem = (int)sizeof(unsigned) * ((kClusterWarps + kClusterCtas) << c.width);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = smem_attr_once(done, reinterpret_cast<const void*>(sort_cluster_kernel<ITEMS>),
+                                 (int)sizeof(unsigned) * ((kClusterWarps + kClusterCtas) << 10));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ITEMS>, c);
+}
+
 int key_bits(long long rows) {   // keys are 0 .. rows
   int b = 1;
   while ((rows >> b) != 0) ++b;
@@ -293,21 +415,40 @@ size_t sort_ids_workspace(long long rows, long long n) {
 }
 
 cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, long long pad, int has_pad, void* ws,
-                     uint2** sorted, cudaStream_t st) {
+                     unsigned* zero, int nzero, uint2** sorted, cudaStream_t st) {
   uint2* buf[2] = {static_cast<uint2*>(ws),
                    reinterpret_cast<uint2*>(static_cast<char*>(ws) + align_up(sizeof(uint2) * (size_t)n))};
   SortArgs a = {};
   a.n = n;
   a.rows = (unsigned)rows;
-  a.tiles = sort_tiles(n);
-  const long long per = (n + a.tiles - 1) / a.tiles;
-  a.span = (per + kSortThreads - 1) / kSortThreads * kSortThreads;
   a.ids = ids;
   a.ids64 = ids64;
   a.pad = pad;
   a.has_pad = has_pad;
+  const int bits = key_bits(rows);
+  if (n <= kClusterMost) {
+    ClusterSortArgs c = {};
+    c.s = a;
+    c.buf[0] = buf[0];
+    c.buf[1] = buf[1];
+    c.passes = (bits + 9) / 10;
+    c.width = (bits + c.passes - 1) / c.passes;
+    c.zero = zero;
+    c.nzero = nzero;
+    *sorted = buf[(c.passes - 1) & 1];
+    if (n <= kBlockMost) return launch_cluster_sort<4>(c, 1, st);
+    if (n <= 4 * kClusterThreads * kClusterCtas) return launch_cluster_sort<4>(c, kClusterCtas, st);
+    return launch_cluster_sort<16>(c, kClusterCtas, st);
+  }
+  if (nzero) {
+    const cudaError_t e = cudaMemsetAsync(zero, 0, sizeof(unsigned) * (size_t)nzero, st);
+    if (e != cudaSuccess) return e;
+  }
+  a.tiles = sort_tiles(n);
+  const long long per = (n + a.tiles - 1) / a.tiles;
+  a.span = (per + kSortThreads - 1) / kSortThreads * kSortThreads;
   a.counts = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 2 * align_up(sizeof(uint2) * (size_t)n));
-  const int bits = key_bits(rows), passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
+  const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
   for (int k = 0; k < passes; ++k) {
     a.shift = k * width;
     a.mask = (1 << width) - 1;
@@ -329,8 +470,11 @@ namespace {
 struct SumArgs {
   long long n, ld_g, ld_w;   // ids; row strides of g and of the table
   unsigned rows;
-  int nv, lg, tile, tiles;   // vectors per row, lanes, positions per tile, tiles
+  int nv, lg, tile;          // vectors per row, lanes of a group, positions per group
+  int blocks;                // blocks along the positions; those behind them set rows to zero
+  int fill;                  // rows per warp of those
   const uint2* sorted;
+  unsigned* arrived;         // [column piece][block]: blocks of the run that starts there
   int mode;                  // scale
   const void* scale;
   double value;
@@ -341,67 +485,128 @@ constexpr int kBatch = 8;
 
 // Stores one finished row; adds its part of ds.
 template <typename T, int V>
-__device__ __forceinline__ void finish_row(const SumArgs& a, unsigned v, int c, const Acc<T>* acc, const T* W, T* dW,
-                                           Acc<T>* ds) {
+__device__ __forceinline__ void finish_row(const SumArgs& a, unsigned v, int c, const Lane<T, V>* acc, const T* W,
+                                           T* dW, Lane<T, V>* ds) {
+  typedef Lane<T, V> L;
   const long long dim = (long long)a.nv * V, col = (long long)c * V;
   if (a.want_ds) {
     const Vec<T, V> w = load_vec<T, V>(W + v * a.ld_w + col);
 #pragma unroll
-    for (int k = 0; k < V; ++k) ds[k] += to_acc(w.v[k]) * acc[k];
+    for (int k = 0; k < lanes<V>; ++k) ds[k] = fma(widen<T, V>(w.v, k), acc[k], ds[k]);
   }
   if (dW) {
     const Acc<T>* s = static_cast<const Acc<T>*>(a.scale) + col;
     Vec<T, V> y;
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      y.v[k] = from_acc<T>(a.mode == kNone ? acc[k] : acc[k] * (a.mode == kValue ? (Acc<T>)a.value : s[k]));
+    for (int k = 0; k < lanes<V>; ++k) {
+      L f = spread<L>((Acc<T>)a.value);
+      if (a.mode == kColumn) f = widen<Acc<T>, V>(s, k);
+      narrow<T, V>(a.mode == kNone ? acc[k] : mul(acc[k], f), y.v, k);
+    }
     store_vec<T, V>(dW + v * dim + col, y);
   }
 }
 
-// Sum of the block's ds over its groups, written as one partial row.
-template <typename T, int V>
-__device__ __forceinline__ void block_ds(const SumArgs& a, int lane, int grp, int ngrp, int c, const Acc<T>* ds,
-                                         Acc<T>* row) {
-  __shared__ Acc<T> red[kThreads];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    __syncthreads();
-    red[threadIdx.x] = ds[k];
-    __syncthreads();
-    if (grp == 0 && c < a.nv) {
-      Acc<T> s = 0;
-      for (int g = 0; g < ngrp; ++g) s += red[(g << a.lg) + lane];
-      row[(long long)c * V + k] = s;
+// Sets the rows that no id names to zero: a warp takes a.fill rows, finds which
+// of them the sorted ids hold (one bisection a lane), and clears the others.
+template <typename T, int V> __device__ __forceinline__ void fill_rows(const SumArgs& a, T* dW) {
+  const int lane = threadIdx.x & 31;
+  const long long warp =
+      (((long long)blockIdx.x - a.blocks) * gridDim.y + blockIdx.y) * (kThreads / 32) + (threadIdx.x >> 5);
+  const long long v0 = warp * a.fill;
+  if (!dW || v0 >= a.rows) return;
+  const long long v = v0 + lane;
+  bool empty = lane < a.fill && v < a.rows;
+  if (empty) {
+    long long lo = 0, hi = a.n;
+    while (lo < hi) {
+      const long long mid = (lo + hi) >> 1;
+      if (a.sorted[mid].x < v) lo = mid + 1;
+      else hi = mid;
     }
+    empty = lo >= a.n || a.sorted[lo].x != v;
+  }
+  const unsigned todo = __ballot_sync(0xffffffffu, empty);
+  const Vec<T, V> zero = {};
+  T* out = dW + v0 * a.nv * V;
+  if (a.nv >= 32) {
+    for (unsigned m = todo; m; m &= m - 1) {
+      T* row = out + (long long)(__ffs(m) - 1) * a.nv * V;
+      for (int c = lane; c < a.nv; c += 32) store_vec<T, V>(row + (long long)c * V, zero);
+    }
+  } else {
+    for (int i = lane; i < a.fill * a.nv; i += 32)
+      if (todo >> (i / a.nv) & 1) store_vec<T, V>(out + (long long)i * V, zero);
   }
 }
 
-// part: two rows of nv * V sums per tile: [0] the run that came in over the
-// tile's left border, [1] the run that starts here and leaves over the right.
+// The block in which the run of `key` that enters block b starts, and the one in
+// which the run that leaves block b (or is in it) ends; by one warp.  `span` is a
+// block's positions.
+__device__ __forceinline__ int run_first(const SumArgs& a, unsigned key, long long span, int b) {
+  const int lane = threadIdx.x & 31;
+  for (int s0 = b - 1;; s0 -= 32) {
+    const int s = s0 - lane;
+    const bool starts = s <= 0 || a.sorted[s * span - 1].x != key;
+    const unsigned m = __ballot_sync(0xffffffffu, starts);
+    if (m) return s0 - (__ffs(m) - 1) > 0 ? s0 - (__ffs(m) - 1) : 0;
+  }
+}
+__device__ __forceinline__ int run_last(const SumArgs& a, unsigned key, long long span, int b) {
+  const int lane = threadIdx.x & 31;
+  for (int e0 = b;; e0 += 32) {
+    const int e = e0 + lane;
+    const bool ends = (e + 1) * span >= a.n || a.sorted[(e + 1) * span].x != key;
+    const unsigned m = __ballot_sync(0xffffffffu, ends);
+    if (m) return e0 + __ffs(m) - 1;
+  }
+}
+
+// part: two rows of sums per block: [0] the run that came in over its left border,
+// [1] the run that starts in it and leaves over the right one.  ds_part: two rows
+// per block: the rows that it finished by itself, and the run that starts in it and
+// crosses blocks (whichever block adds that up).
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __restrict__ g, const T* __restrict__ W,
-                                                       T* __restrict__ dW, Acc<T>* __restrict__ part,
-                                                       Acc<T>* __restrict__ ds_part) {
+                                                       T* __restrict__ dW, Acc<T>* part, Acc<T>* ds_part) {
+  typedef Acc<T> A;
+  typedef Lane<T, V> L;
+  constexpr int N = lanes<V>;
+  __shared__ __align__(16) A head[kThreads * V], tail[kThreads * V];
+  __shared__ int flags[kThreads];      // per group
+  __shared__ int cross[6];             // first and last block of the two crossing runs; whether to add them up
+  griddep_wait();
+  if ((int)blockIdx.x >= a.blocks) {
+    fill_rows<T, V>(a, dW);
+    return;
+  }
+  enum { kCameIn = 1, kGoesOn = 2, kSingle = 4 };
   const int lane = threadIdx.x & ((1 << a.lg) - 1);
   const int grp = threadIdx.x >> a.lg, ngrp = kThreads >> a.lg;
   const int c = (blockIdx.y << a.lg) + lane;
-  const long long t = (long long)blockIdx.x * ngrp + grp;
-  const long long dim = (long long)a.nv * V;
-  Acc<T> ds[V];
+  const long long dim = (long long)a.nv * V, col = (long long)c * V;
+  const long long span = (long long)ngrp * a.tile;
+  const long long b0 = blockIdx.x * span, b1 = b0 + span < a.n ? b0 + span : a.n;
+  const long long p0 = b0 + (long long)grp * a.tile, p1 = p0 + a.tile < a.n ? p0 + a.tile : a.n;
+  const bool there = p0 < a.n, on = there && c < a.nv;
+  const L zero = spread<L>((A)0);
+  L ds[N];
 #pragma unroll
-  for (int k = 0; k < V; ++k) ds[k] = 0;
-  const bool on = t < a.tiles && c < a.nv;
-  const long long p0 = t * a.tile;
-  const long long p1 = p0 + a.tile < a.n ? p0 + a.tile : a.n;
-  if (on) {
-    const unsigned before = p0 > 0 ? a.sorted[p0 - 1].x : 0xffffffffu;
-    const unsigned after = p1 < a.n ? a.sorted[p1].x : 0xffffffffu;
-    Acc<T> acc[V];
+  for (int k = 0; k < N; ++k) ds[k] = zero;
+  unsigned first = a.rows, last = a.rows;
+  int mine = 0;
+  if (there) {
+    first = a.sorted[p0].x;
+    last = a.sorted[p1 - 1].x;
+    mine = (first < a.rows && p0 > 0 && a.sorted[p0 - 1].x == first ? kCameIn : 0) |
+           (last < a.rows && p1 < a.n && a.sorted[p1].x == last ? kGoesOn : 0) | (first == last ? kSingle : 0);
+  }
+  if (on && first < a.rows) {
+    L acc[N];
 #pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0;
-    unsigned cur = a.sorted[p0].x;
-    bool came_in = cur == before;
+    for (int k = 0; k < N; ++k) acc[k] = zero;
+    unsigned cur = first;
+    bool came_in = mine & kCameIn;
     for (long long p = p0; p < p1 && cur < a.rows; p += kBatch) {
       uint2 kv[kBatch];
       Vec<T, V> x[kBatch];
@@ -409,167 +614,210 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
       for (int u = 0; u < kBatch; ++u) kv[u] = p + u < p1 ? a.sorted[p + u] : make_uint2(a.rows, 0);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (kv[u].x < a.rows) x[u] = load_vec<T, V>(g + kv[u].y * a.ld_g + (long long)c * V);
+        if (kv[u].x < a.rows) x[u] = load_vec<T, V>(g + kv[u].y * a.ld_g + col);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        if (kv[u].x != cur) {
-          if (p + u < p1) {   // the run of `cur` ends inside the tile
-            if (came_in) {
-              Acc<T>* o = part + 2 * t * dim + (long long)c * V;
+        if (kv[u].x != cur && p + u < p1) {   // the run of `cur` ends inside the tile
+          if (came_in) {
 #pragma unroll
-              for (int k = 0; k < V; ++k) o[k] = acc[k];
-            } else if (cur < a.rows) {
-              finish_row<T, V>(a, cur, c, acc, W, dW, ds);
-            }
-            came_in = false;
-            cur = kv[u].x;
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] = 0;
+            for (int k = 0; k < N; ++k) narrow<A, V>(acc[k], head + threadIdx.x * V, k);
+          } else if (cur < a.rows) {
+            finish_row<T, V>(a, cur, c, acc, W, dW, ds);
           }
+          came_in = false;
+          cur = kv[u].x;
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] = zero;
         }
         if (kv[u].x < a.rows) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) acc[k] += to_acc(x[u].v[k]);
+          for (int k = 0; k < N; ++k) acc[k] = add(acc[k], widen<T, V>(x[u].v, k));
         }
       }
     }
-    if (cur < a.rows) {   // the last run of the tile
-      if (came_in || cur == after) {
-        Acc<T>* o = part + (2 * t + (came_in ? 0 : 1)) * dim + (long long)c * V;
+    if (cur < a.rows) {   // the tile's last run
+      if (came_in) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = acc[k];
+        for (int k = 0; k < N; ++k) narrow<A, V>(acc[k], head + threadIdx.x * V, k);
+      } else if (mine & kGoesOn) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) narrow<A, V>(acc[k], tail + threadIdx.x * V, k);
       } else {
         finish_row<T, V>(a, cur, c, acc, W, dW, ds);
       }
     }
   }
-  if (a.want_ds) block_ds<T, V>(a, lane, grp, ngrp, c, ds, ds_part + blockIdx.x * dim);
-}
+  if (lane == 0) flags[grp] = mine;
+  __syncthreads();
 
-// First position of the sorted pairs with a key above `key`, in [lo, n).
-__device__ __forceinline__ long long run_end(const uint2* sorted, long long lo, long long n, unsigned key) {
-  long long hi = n;
-  while (lo < hi) {
-    const long long mid = (lo + hi) >> 1;
-    if (sorted[mid].x <= key) lo = mid + 1;
-    else hi = mid;
+  // Runs that cross the block's tiles: the group in which one starts adds up the
+  // heads of those behind it; the run that came into the block is group 0's too.
+  A* mine_part = part + (long long)blockIdx.x * 2 * dim;
+  const bool through = (mine & (kCameIn | kSingle | kGoesOn)) == (kCameIn | kSingle | kGoesOn);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const bool starts = which == 0 ? grp == 0 && (mine & kCameIn) : (mine & kGoesOn) && !((mine & kCameIn) && (mine & kSingle));
+    if (on && starts) {
+      L acc[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = widen<A, V>((which ? tail : head) + threadIdx.x * V, k);
+      bool more = which ? true : through;
+      int q = grp + 1;
+      for (; more && q < ngrp && b0 + (long long)q * a.tile < a.n; ++q) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = add(acc[k], widen<A, V>(head + ((q << a.lg) + lane) * V, k));
+        more = (flags[q] & (kSingle | kGoesOn)) == (kSingle | kGoesOn);
+      }
+      if (which == 0 || more) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) narrow<A, V>(acc[k], mine_part + which * dim + col, k);
+      } else {
+        finish_row<T, V>(a, last, c, acc, W, dW, ds);
+      }
+    }
   }
-  return lo;
-}
 
-// The runs that cross tile borders: a block takes the run that starts in tile
-// t and leaves it, its groups sum contiguous parts of the list of partial
-// rows, and the groups' sums are added in order.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) join_kernel(SumArgs a, const T* __restrict__ W, T* __restrict__ dW,
-                                                        const Acc<T>* __restrict__ part,
-                                                        Acc<T>* __restrict__ ds_part) {
-  __shared__ Acc<T> red[kThreads * V];
-  const int lane = threadIdx.x & ((1 << a.lg) - 1);
-  const int grp = threadIdx.x >> a.lg, ngrp = kThreads >> a.lg;
-  const int c = (blockIdx.y << a.lg) + lane;
-  const long long dim = (long long)a.nv * V;
-  Acc<T> ds[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) ds[k] = 0;
-  for (long long t = blockIdx.x; t + 1 < a.tiles; t += gridDim.x) {
-    const long long p0 = t * a.tile, p1 = p0 + a.tile;
-    const unsigned key = a.sorted[p1].x;
-    if (key >= a.rows || a.sorted[p1 - 1].x != key) continue;            // no run leaves tile t
-    if (p0 > 0 && a.sorted[p0 - 1].x == key) continue;                   // it started in an earlier tile
-    const long long end = run_end(a.sorted, p1, a.n, key);
-    const long long last = (end - 1) / a.tile;                           // partial rows t, t + 1 .. last
-    const long long count = last - t + 1, each = (count + ngrp - 1) / ngrp;
-    Acc<T> acc[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0;
-    if (c < a.nv) {
-      const long long e = (grp + 1) * each < count ? (grp + 1) * each : count;
-#pragma unroll 4
-      for (long long i = grp * each; i < e; ++i) {
-        const Acc<T>* o = part + (2 * (t + i) + (i == 0 ? 1 : 0)) * dim + (long long)c * V;
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += o[k];
+  // Runs that cross blocks
+  const unsigned key_in = a.sorted[b0].x, key_out = a.sorted[b1 - 1].x;
+  const bool enters = b0 > 0 && key_in < a.rows && a.sorted[b0 - 1].x == key_in;
+  const bool leaves = b1 < a.n && key_out < a.rows && a.sorted[b1].x == key_out;
+  const bool starts_here = leaves && !(enters && key_in == key_out);
+  if (enters || starts_here) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int f = enters ? run_first(a, key_in, span, blockIdx.x) : 0, e = enters ? run_last(a, key_in, span, blockIdx.x) : 0;
+      const int e2 = starts_here ? run_last(a, key_out, span, blockIdx.x) : 0;
+      if (threadIdx.x == 0) {
+        unsigned* n = a.arrived + (size_t)blockIdx.y * a.blocks;
+        cross[0] = f;
+        cross[1] = e;
+        cross[2] = enters && atomicAdd(n + f, 1u) == (unsigned)(e - f);
+        cross[3] = blockIdx.x;
+        cross[4] = e2;
+        cross[5] = starts_here && atomicAdd(n + blockIdx.x, 1u) == (unsigned)(e2 - (int)blockIdx.x);
       }
     }
     __syncthreads();
+    __threadfence();
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      if (!cross[3 * which + 2]) continue;
+      const int f = cross[3 * which], count = cross[3 * which + 1] - f + 1, each = (count + ngrp - 1) / ngrp;
+      L acc[N], join[N];
 #pragma unroll
-    for (int k = 0; k < V; ++k) red[threadIdx.x * V + k] = acc[k];
+      for (int k = 0; k < N; ++k) acc[k] = join[k] = zero;
+      if (c < a.nv) {
+        const int to = (grp + 1) * each < count ? (grp + 1) * each : count;
+#pragma unroll 4
+        for (int i = grp * each; i < to; ++i) {
+          const A* o = part + ((long long)(f + i) * 2 + (i == 0 ? 1 : 0)) * dim + col;
+          A v[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] = __ldcg(o + k);
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] = add(acc[k], widen<A, V>(v, k));
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < N; ++k) narrow<A, V>(acc[k], head + threadIdx.x * V, k);
+      __syncthreads();
+      if (grp == 0 && c < a.nv) {
+        for (int q = 1; q < ngrp; ++q) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] = add(acc[k], widen<A, V>(head + ((q << a.lg) + lane) * V, k));
+        }
+        finish_row<T, V>(a, which ? key_out : key_in, c, acc, W, dW, join);
+        if (a.want_ds) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) narrow<A, V>(join[k], ds_part + ((long long)f * 2 + 1) * dim + col, k);
+        }
+      }
+    }
+  }
+  if (a.want_ds) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) narrow<A, V>(ds[k], head + threadIdx.x * V, k);
     __syncthreads();
     if (grp == 0 && c < a.nv) {
       for (int q = 1; q < ngrp; ++q) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += red[((q << a.lg) + lane) * V + k];
+        for (int k = 0; k < N; ++k) ds[k] = add(ds[k], widen<A, V>(head + ((q << a.lg) + lane) * V, k));
       }
-      finish_row<T, V>(a, key, c, acc, W, dW, ds);
+      A* o = ds_part + (long long)blockIdx.x * 2 * dim + col;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        narrow<A, V>(ds[k], o, k);
+        if (!starts_here) narrow<A, V>(zero, o + dim, k);
+      }
     }
   }
-  if (a.want_ds) block_ds<T, V>(a, lane, grp, ngrp, c, ds, ds_part + blockIdx.x * dim);
-}
-
-// How the sorted positions are cut: 32 to a tile, a power of two more when
-// that would leave over 2^16 tiles.
-int sum_tile(long long n) {
-  int t = 32;
-  while (n / t > 65536) t *= 2;
-  return t;
 }
 
 struct SumPlan {
-  int tile, tiles, lg, cols, blocks, join;   // cols: column pieces; blocks, join: blocks along the tiles
+  int lg, cols, tile, blocks, fill, fill_blocks;
 };
 
-SumPlan sum_plan(long long n, int nv) {
+// Tiles of 4 to 32 positions (more where that would leave over 2^16 blocks): as
+// long as they leave four blocks a SM.
+constexpr int kSms = 148;   // of a B200
+
+SumPlan sum_plan(long long n, long long rows, int nv) {
   SumPlan p;
-  p.tile = sum_tile(n);
-  p.tiles = (int)((n + p.tile - 1) / p.tile);
   p.lg = 0;
   while (p.lg < 5 && (1 << p.lg) < nv) ++p.lg;
   p.cols = (nv + (1 << p.lg) - 1) >> p.lg;
   const int ngrp = kThreads >> p.lg;
-  p.blocks = (p.tiles + ngrp - 1) / ngrp;
-  p.join = p.tiles < 1024 ? p.tiles : 1024;
+  p.tile = 4;
+  while ((p.tile < 32 && n * p.cols > 2LL * p.tile * ngrp * 4 * kSms) || n / ((long long)p.tile * ngrp) > 65536) p.tile *= 2;
+  p.blocks = (int)((n + (long long)p.tile * ngrp - 1) / ((long long)p.tile * ngrp));
+  // rows of a warp: 32 short ones, fewer as they grow
+  p.fill = nv >= 128 ? 8 : nv >= 32 ? 16 : 32;
+  const long long warps = (rows + p.fill - 1) / p.fill, per = (long long)(kThreads / 32) * p.cols;
+  p.fill_blocks = (int)((warps + per - 1) / per);
   return p;
 }
 
 struct ScatterLayout {
-  size_t sort, part, ds, total;
+  size_t sort, arrived, part, ds, total;
 };
 
-// Sizes do not depend on the addresses: the vector may be as narrow as one
-// element, which has the most column pieces and the same rows.
+// Room for any vector width that the addresses allow.
 ScatterLayout scatter_layout(long long rows, int dim, int dtype, long long n, int want_ds) {
-  const SumPlan p1 = sum_plan(n, dim);
-  const int es = acc_size(dtype);
+  const int es = acc_size(dtype), widest = 16 / elem_size(dtype);
+  size_t blocks = 0, pieces = 0;
+  for (int v = 1; v <= widest; v *= 2) {
+    if (dim % v) break;
+    const SumPlan p = sum_plan(n, rows, dim / v);
+    if ((size_t)p.blocks > blocks) blocks = p.blocks;
+    if ((size_t)p.blocks * p.cols > pieces) pieces = (size_t)p.blocks * p.cols;
+  }
   ScatterLayout l;
   l.sort = align_up(sort_ids_workspace(rows, n));
-  l.part = align_up((size_t)2 * p1.tiles * dim * es);
-  // partial rows of ds: the fewest groups per block (32 lanes) give the most blocks
-  const size_t blocks = (size_t)(p1.tiles + 7) / 8 + 1024;
-  l.ds = want_ds ? align_up(blocks * dim * es) : 0;
-  l.total = l.sort + l.part + l.ds;
+  l.arrived = align_up(sizeof(unsigned) * pieces);
+  l.part = align_up(blocks * 2 * dim * es);
+  l.ds = want_ds ? align_up(blocks * 2 * dim * es) : 0;
+  l.total = l.sort + l.arrived + l.part + l.ds;
   return l;
 }
 
 template <typename T, int V>
 cudaError_t scatter_launch(SumArgs a, int dim, const T* g, const T* W, T* dW, void* d_scale, char* part, char* ds,
-                           cudaStream_t st) {
-  const SumPlan p = sum_plan(a.n, dim / V);
+                           const SumPlan& p, cudaStream_t st) {
   a.nv = dim / V;
   a.lg = p.lg;
   a.tile = p.tile;
-  a.tiles = p.tiles;
+  a.blocks = p.blocks;
+  a.fill = p.fill;
   Acc<T>* pt = reinterpret_cast<Acc<T>*>(part);
   Acc<T>* dp = reinterpret_cast<Acc<T>*>(ds);
-  sum_kernel<T, V><<<dim3(p.blocks, p.cols), kThreads, 0, st>>>(a, g, W, dW, pt, dp);
-  int rows = p.blocks;
-  if (p.tiles > 1) {
-    join_kernel<T, V><<<dim3(p.join, p.cols), kThreads, 0, st>>>(a, W, dW, pt, dp + (size_t)rows * dim);
-    rows += p.join;
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && a.want_ds) e = column_sum(dp, rows, dim, dim, static_cast<Acc<T>*>(d_scale), st);
-  return e;
+  const int fill = dW ? p.fill_blocks : 0;
+  const cudaError_t e = launch_pdl(sum_kernel<T, V>, dim3(p.blocks + fill, p.cols), dim3(kThreads), 0, st, a, g, W, dW,
+                                   pt, dp);
+  if (e != cudaSuccess || !a.want_ds) return e;
+  return column_sum(dp, 2 * p.blocks, dim, dim, static_cast<Acc<T>*>(d_scale), st);
 }
 
 bool rows_args_ok(long long rows, int dim, int dtype, long long n, const void* ids, int mode, const void* scale) {
@@ -642,21 +890,6 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
   if (ws_bytes < l.total) return bad_args("lg_rows_scatter: workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* w = static_cast<char*>(ws);
-  SumArgs a = {};
-  a.n = n;
-  a.ld_g = ld_g;
-  a.ld_w = ld_table;
-  a.rows = (unsigned)rows;
-  a.mode = scale_mode;
-  a.scale = scale;
-  a.value = scale_value;
-  a.want_ds = d_scale != nullptr;
-  uint2* sorted = nullptr;
-  cudaError_t e = sort_ids(rows, n, ids, ids64, padding, has_padding, w, &sorted, st);
-  if (e == cudaSuccess && d_table)
-    e = cudaMemsetAsync(d_table, 0, (size_t)rows * dim * elem_size(dtype), st);
-  if (e != cudaSuccess) return cuda_status(e, "lg_rows_scatter");
-  a.sorted = sorted;
   Align al(elem_size(dtype));
   al.address(g);
   al.elements(ld_g);
@@ -667,10 +900,25 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
     al.elements(ld_table);
   }
   const int vec = al.vec();
+  const SumPlan p = sum_plan(n, rows, dim / vec);
+  SumArgs a = {};
+  a.n = n;
+  a.ld_g = ld_g;
+  a.ld_w = ld_table;
+  a.rows = (unsigned)rows;
+  a.mode = scale_mode;
+  a.scale = scale;
+  a.value = scale_value;
+  a.want_ds = d_scale != nullptr;
+  a.arrived = reinterpret_cast<unsigned*>(w + l.sort);
+  uint2* sorted = nullptr;
+  const cudaError_t e = sort_ids(rows, n, ids, ids64, padding, has_padding, w, a.arrived, p.blocks * p.cols, &sorted, st);
+  if (e != cudaSuccess) return cuda_status(e, "lg_rows_scatter");
+  a.sorted = sorted;
   auto run = [&]() -> cudaError_t {
 #define LG_F(T, V)                                                                                                  \
   scatter_launch<T, V>(a, dim, static_cast<const T*>(g), static_cast<const T*>(table), static_cast<T*>(d_table), \
-                       d_scale, w + l.sort, w + l.sort + l.part, st)
+                       d_scale, w + l.sort + l.arrived, w + l.sort + l.arrived + l.part, p, st)
     LG_ROWS_DISPATCH(LG_F)
 #undef LG_F
   };
