@@ -6,7 +6,10 @@ Every CUDA source under csrc/ is compiled by nvcc for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a) with -lineinfo, then linked into
 gpu_eigsh/_lib/liblanczos_b200.so against the static CUDA runtime, so the
 library carries no dependency beyond the driver.  Objects go to _build/.
-Rebuilds only what changed (any header change rebuilds everything).
+Then csrc/torch/features.cpp, the torch binding of the node-feature operators,
+is compiled by g++ against the installed torch and that library into
+gpu_eigsh/_lib/_torch_features.so.  Rebuilds only what changed (any header
+change rebuilds everything).
 """
 from __future__ import annotations
 
@@ -23,6 +26,8 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 OUT_DIR = PKG / "gpu_eigsh" / "_lib"
 LIB = OUT_DIR / "liblanczos_b200.so"
+TORCH_SRC = CSRC / "torch" / "features.cpp"
+TORCH_LIB = OUT_DIR / "_torch_features.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -37,6 +42,33 @@ def nvcc() -> str:
         if cand and Path(cand).exists():
             return cand
     raise RuntimeError("nvcc not found")
+
+
+def host_compiler() -> str:
+    """A g++ with a shared libstdc++: one that links its own copy into the binding
+    crashes where torch's objects cross between the two."""
+    for cand in (shutil.which("g++"), "/usr/bin/g++", os.environ.get("CXX")):
+        if cand and Path(cand).exists():
+            res = subprocess.run([cand, "-print-file-name=libstdc++.so"], capture_output=True, text=True)
+            if os.path.isabs(res.stdout.strip()):
+                return cand
+    raise RuntimeError("no g++ with a shared libstdc++ found")
+
+
+def torch_binding_command() -> list[str]:
+    """g++ line of the torch binding (torch's own include and library paths)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cuda = Path(nvcc()).resolve().parents[1]
+    inc = [*include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
+    return [host_compiler(), "-std=c++17", "-O2", "-fPIC", "-shared",
+            "-DTORCH_EXTENSION_NAME=_torch_features", "-DTORCH_API_INCLUDE_EXTENSION_H",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
+            str(TORCH_SRC), "-o", str(TORCH_LIB), *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch",
+            "-ltorch_cpu", "-ltorch_python", f"-L{OUT_DIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
 
 
 def _newest(paths) -> float:
@@ -85,6 +117,15 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
+
+    if force or not TORCH_LIB.exists() or TORCH_LIB.stat().st_mtime < _newest([TORCH_SRC, *INCLUDE.glob("*.h")]):
+        cmd = torch_binding_command()
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("g++ failed for csrc/torch/features.cpp")
     return LIB
 
 

@@ -162,7 +162,7 @@ constexpr int kMaxTiles = 296;
 struct SortArgs {
   long long n, span;       // span: keys of one block, a multiple of kSortThreads
   unsigned rows;
-  int shift, mask, tiles;
+  int shift, mask, width, tiles;
   const void* ids;         // first pass: the ids themselves
   int ids64, has_pad;
   long long pad;
@@ -178,6 +178,23 @@ __device__ __forceinline__ uint2 sort_pair(const SortArgs& a, long long p) {
   return make_uint2(ok ? (unsigned)id : a.rows, (unsigned)p);
 }
 
+// The lanes whose digit (width bits) equals this lane's, among those that are
+// `in`; by one vote a bit.  All lanes of the warp vote, always: a vote or a
+// __syncwarp of some of them costs about 40 cycles more (131,072 ids in one
+// cluster: 88 us with them).
+__device__ __forceinline__ unsigned equal_lanes(bool in, unsigned digit, int width) {
+  unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    if (b < width) {
+      const bool bit = digit >> b & 1u;
+      const unsigned vote = __ballot_sync(0xffffffffu, bit);
+      same &= bit ? vote : ~vote;
+    }
+  }
+  return same;
+}
+
 // Digit counts of the block's span, per warp, in shared memory.
 __device__ __forceinline__ void sort_count(const SortArgs& a, unsigned (*cnt)[kDigits]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -185,9 +202,18 @@ __device__ __forceinline__ void sort_count(const SortArgs& a, unsigned (*cnt)[kD
   __syncthreads();
   const long long part = a.span / kSortWarps;
   const long long p0 = blockIdx.x * a.span + warp * part;
-  for (long long i = 0; i < part; i += 32) {
-    const long long p = p0 + i + lane;
-    if (p < a.n) atomicAdd(&cnt[warp][(sort_pair(a, p).x >> a.shift) & a.mask], 1u);
+  for (long long i = 0; i < part; i += 128) {
+    unsigned key[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long p = p0 + i + 32 * u + lane;
+      key[u] = i + 32 * u < part && p < a.n ? sort_pair(a, p).x : 0xffffffffu;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long p = p0 + i + 32 * u + lane;
+      if (i + 32 * u < part && p < a.n) atomicAdd(&cnt[warp][(key[u] >> a.shift) & a.mask], 1u);
+    }
   }
   __syncthreads();
 }
@@ -223,7 +249,7 @@ __global__ void __launch_bounds__(32) sort_scan_kernel(SortArgs a) {
   if (threadIdx.x == 0) a.counts[(size_t)kDigits * a.tiles + blockIdx.x] = run;
 }
 
-// Exclusive prefix over kDigits values, one per thread (256 threads).
+// Exclusive prefix over the values of the block's threads.
 __device__ __forceinline__ unsigned digit_prefix(unsigned v, unsigned* scratch) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned s = v;
@@ -234,9 +260,13 @@ __device__ __forceinline__ unsigned digit_prefix(unsigned v, unsigned* scratch) 
   }
   if (lane == 31) scratch[warp] = s;
   __syncthreads();
-  unsigned base = 0;
-  for (int w = 0; w < warp; ++w) base += scratch[w];
-  return base + s - v;
+  unsigned t = lane < (int)(blockDim.x >> 5) ? scratch[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned u = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) t += u;
+  }
+  return (warp ? __shfl_sync(0xffffffffu, t, warp - 1) : 0) + s - v;
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) {
@@ -262,19 +292,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
   for (long long i = 0; i < part; i += 32) {
     const long long p = p0 + i + lane;
     const bool in = p < a.n;
-    const unsigned act = __ballot_sync(0xffffffffu, in);
-    if (!act) break;
-    if (in) {
-      const uint2 kv = sort_pair(a, p);
-      const unsigned dg = (kv.x >> a.shift) & a.mask;
-      const unsigned peers = __match_any_sync(act, dg);
-      const unsigned rank = __popc(peers & ((1u << lane) - 1));
-      const unsigned at = cnt[warp][dg];
-      __syncwarp(act);
-      if (rank == 0) cnt[warp][dg] = at + __popc(peers);
-      __syncwarp(act);
-      a.out[at + rank] = kv;
-    }
+    const uint2 kv = in ? sort_pair(a, p) : make_uint2(0, 0);
+    const unsigned dg = (kv.x >> a.shift) & a.mask;
+    const unsigned peers = equal_lanes(in, dg, a.width);
+    const unsigned rank = __popc(peers & ((1u << lane) - 1));
+    const unsigned at = cnt[warp][dg];
+    __syncwarp();
+    if (in && rank == 0) cnt[warp][dg] = at + __popc(peers);
+    __syncwarp();
+    if (in) a.out[at + rank] = kv;
   }
 }
 
@@ -328,22 +354,21 @@ __global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(Cluste
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const unsigned act = __ballot_sync(0xffffffffu, p0 + 32 * i < a.n);
-      if (p0 + 32 * i < a.n) {
-        const unsigned d = (kv[i].x >> shift) & mask;
-        const unsigned peers = __match_any_sync(act, d);
-        const unsigned rank = __popc(peers & ((1u << lane) - 1));
-        const unsigned at = own[d];
-        __syncwarp(act);
-        if (rank == 0) own[d] = at + __popc(peers);
-        __syncwarp(act);
-        place[i] = at + rank;
-      }
+      const bool in = p0 + 32 * i < a.n;
+      const unsigned d = (kv[i].x >> shift) & mask;
+      const unsigned peers = equal_lanes(in, d, c.width);
+      const unsigned rank = __popc(peers & ((1u << lane) - 1));
+      const unsigned at = own[d];
+      __syncwarp();
+      if (in && rank == 0) own[d] = at + __popc(peers);
+      __syncwarp();
+      place[i] = at + rank;
     }
     __syncthreads();
     const int d = threadIdx.x;
     unsigned total = 0;
     if (d < digits) {
+#pragma unroll
       for (int w = 0; w < kClusterWarps; ++w) total += smem[w * digits + d];
       for (int q = 0; q < ctas; ++q) cluster.map_shared_rank(all, q)[me * digits + d] = total;
     }
@@ -359,10 +384,16 @@ __global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(Cluste
     }
     unsigned base = digit_prefix(total, scratch) + below;
     if (d < digits) {
-      for (int w = 0; w < kClusterWarps; ++w) {
-        const unsigned v = smem[w * digits + d];
-        smem[w * digits + d] = base;
-        base += v;
+#pragma unroll
+      for (int w0 = 0; w0 < kClusterWarps; w0 += 8) {
+        unsigned v[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v[w] = smem[(w0 + w) * digits + d];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          smem[(w0 + w) * digits + d] = base;
+          base += v[w];
+        }
       }
     }
     __syncthreads();
@@ -372,6 +403,28 @@ __global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(Cluste
       if (p0 + 32 * i < a.n) out[own[(kv[i].x >> shift) & mask] + place[i]] = kv[i];
     cluster.sync();   // the pairs are in memory, and `all` may be written again
   }
+}
+
+// Up to kSmallMost ids: every thread counts the pairs before its own, which is the
+// place of its pair.  One read of shared memory serves four comparisons of a warp.
+constexpr int kSmallMost = 512;
+
+__global__ void __launch_bounds__(kSmallMost) sort_small_kernel(ClusterSortArgs c) {
+  __shared__ __align__(16) unsigned key[kSmallMost];
+  for (int i = threadIdx.x; i < c.nzero; i += kSmallMost) c.zero[i] = 0;
+  const int p = threadIdx.x, n = (int)c.s.n;
+  uint2 kv = make_uint2(0xffffffffu, 0);
+  if (p < n) kv = sort_pair(c.s, p);
+  key[p] = kv.x;
+  __syncthreads();
+  if (p >= n) return;
+  int place = 0;
+  for (int i = 0; i < n; i += 4) {
+    const uint4 k = *reinterpret_cast<const uint4*>(key + i);
+    place += (k.x < kv.x || (k.x == kv.x && i < p)) + (k.y < kv.x || (k.y == kv.x && i + 1 < p)) +
+             (k.z < kv.x || (k.z == kv.x && i + 2 < p)) + (k.w < kv.x || (k.w == kv.x && i + 3 < p));
+  }
+  c.buf[0][place] = kv;
 }
 
 template <int ITEMS> cudaError_t launch_cluster_sort(const ClusterSortArgs& c, int ctas, cudaStream_t st) {
@@ -435,6 +488,11 @@ cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, lo
     c.width = (bits + c.passes - 1) / c.passes;
     c.zero = zero;
     c.nzero = nzero;
+    if (n <= kSmallMost) {
+      *sorted = buf[0];
+      sort_small_kernel<<<1, kSmallMost, 0, st>>>(c);
+      return cudaGetLastError();
+    }
     *sorted = buf[(c.passes - 1) & 1];
     if (n <= kBlockMost) return launch_cluster_sort<4>(c, 1, st);
     if (n <= 4 * kClusterThreads * kClusterCtas) return launch_cluster_sort<4>(c, kClusterCtas, st);
@@ -452,6 +510,7 @@ cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, lo
   for (int k = 0; k < passes; ++k) {
     a.shift = k * width;
     a.mask = (1 << width) - 1;
+    a.width = width;
     a.in = k ? buf[(k - 1) & 1] : nullptr;
     a.out = buf[k & 1];
     sort_count_kernel<<<a.tiles, kSortThreads, 0, st>>>(a);
@@ -508,35 +567,42 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned v, int c, 
 }
 
 // Sets the rows that no id names to zero: a warp takes a.fill rows, finds which
-// of them the sorted ids hold (one bisection a lane), and clears the others.
-template <typename T, int V> __device__ __forceinline__ void fill_rows(const SumArgs& a, T* dW) {
+// of them the sorted ids hold (one bisection a lane), and clears the others, each
+// run of consecutive ones as one range of bytes, so that the row length does not
+// matter to the width of the stores.
+template <typename T> __device__ __forceinline__ void fill_rows(const SumArgs& a, long long dim, long long block, T* dW) {
   const int lane = threadIdx.x & 31;
-  const long long warp =
-      (((long long)blockIdx.x - a.blocks) * gridDim.y + blockIdx.y) * (kThreads / 32) + (threadIdx.x >> 5);
-  const long long v0 = warp * a.fill;
-  if (!dW || v0 >= a.rows) return;
+  const long long v0 = (block * (kThreads / 32) + (threadIdx.x >> 5)) * a.fill;
+  if (v0 >= a.rows) return;
   const long long v = v0 + lane;
   bool empty = lane < a.fill && v < a.rows;
   if (empty) {
-    long long lo = 0, hi = a.n;
+    unsigned lo = 0, hi = (unsigned)a.n;
     while (lo < hi) {
-      const long long mid = (lo + hi) >> 1;
+      const unsigned mid = (lo + hi) >> 1;
       if (a.sorted[mid].x < v) lo = mid + 1;
       else hi = mid;
     }
     empty = lo >= a.n || a.sorted[lo].x != v;
   }
-  const unsigned todo = __ballot_sync(0xffffffffu, empty);
-  const Vec<T, V> zero = {};
-  T* out = dW + v0 * a.nv * V;
-  if (a.nv >= 32) {
-    for (unsigned m = todo; m; m &= m - 1) {
-      T* row = out + (long long)(__ffs(m) - 1) * a.nv * V;
-      for (int c = lane; c < a.nv; c += 32) store_vec<T, V>(row + (long long)c * V, zero);
-    }
-  } else {
-    for (int i = lane; i < a.fill * a.nv; i += 32)
-      if (todo >> (i / a.nv) & 1) store_vec<T, V>(out + (long long)i * V, zero);
+  unsigned todo = __ballot_sync(0xffffffffu, empty);
+  while (todo) {
+    const int first = __ffs(todo) - 1;
+    const unsigned rest = ~(todo >> first);
+    const int count = rest ? __ffs(rest) - 1 : 32;   // of consecutive rows (a shift by 32 - first fills with zeros)
+    todo &= count + first >= 32 ? (1u << first) - 1u : ~(((1u << count) - 1u) << first);
+    T* p = dW + (v0 + first) * dim;
+    T* const end = p + count * dim;
+    const T zero = from_acc<T>((Acc<T>)0);
+    // up to the next multiple of 16 bytes, whole vectors, the rest
+    const int skip = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+    if (lane < skip && p + lane < end) p[lane] = zero;
+    p += skip;
+    const long long vecs = end > p ? (end - p) / (16 / (long long)sizeof(T)) : 0;
+    uint4* q = reinterpret_cast<uint4*>(p);
+    for (long long i = lane; i < vecs; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+    p += vecs * (16 / sizeof(T));
+    if (p + lane < end) p[lane] = zero;
   }
 }
 
@@ -576,8 +642,12 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
   __shared__ int flags[kThreads];      // per group
   __shared__ int cross[6];             // first and last block of the two crossing runs; whether to add them up
   griddep_wait();
-  if ((int)blockIdx.x >= a.blocks) {
-    fill_rows<T, V>(a, dW);
+  // The blocks that sum and those that clear rows alternate, so that the ones'
+  // waits for loads run beside the others' stores.
+  const long long most = gridDim.x;
+  const int block = (int)((long long)blockIdx.x * a.blocks / most);
+  if ((int)(((long long)blockIdx.x + 1) * a.blocks / most) == block) {
+    fill_rows<T>(a, (long long)a.nv * V, ((long long)blockIdx.x - block) * gridDim.y + blockIdx.y, dW);
     return;
   }
   enum { kCameIn = 1, kGoesOn = 2, kSingle = 4 };
@@ -586,7 +656,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
   const int c = (blockIdx.y << a.lg) + lane;
   const long long dim = (long long)a.nv * V, col = (long long)c * V;
   const long long span = (long long)ngrp * a.tile;
-  const long long b0 = blockIdx.x * span, b1 = b0 + span < a.n ? b0 + span : a.n;
+  const long long b0 = block * span, b1 = b0 + span < a.n ? b0 + span : a.n;
   const long long p0 = b0 + (long long)grp * a.tile, p1 = p0 + a.tile < a.n ? p0 + a.tile : a.n;
   const bool there = p0 < a.n, on = there && c < a.nv;
   const L zero = spread<L>((A)0);
@@ -652,7 +722,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
 
   // Runs that cross the block's tiles: the group in which one starts adds up the
   // heads of those behind it; the run that came into the block is group 0's too.
-  A* mine_part = part + (long long)blockIdx.x * 2 * dim;
+  A* mine_part = part + (long long)block * 2 * dim;
   const bool through = (mine & (kCameIn | kSingle | kGoesOn)) == (kCameIn | kSingle | kGoesOn);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -686,16 +756,16 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
     __threadfence();
     __syncthreads();
     if (threadIdx.x < 32) {
-      const int f = enters ? run_first(a, key_in, span, blockIdx.x) : 0, e = enters ? run_last(a, key_in, span, blockIdx.x) : 0;
-      const int e2 = starts_here ? run_last(a, key_out, span, blockIdx.x) : 0;
+      const int f = enters ? run_first(a, key_in, span, block) : 0, e = enters ? run_last(a, key_in, span, block) : 0;
+      const int e2 = starts_here ? run_last(a, key_out, span, block) : 0;
       if (threadIdx.x == 0) {
         unsigned* n = a.arrived + (size_t)blockIdx.y * a.blocks;
         cross[0] = f;
         cross[1] = e;
         cross[2] = enters && atomicAdd(n + f, 1u) == (unsigned)(e - f);
-        cross[3] = blockIdx.x;
+        cross[3] = block;
         cross[4] = e2;
-        cross[5] = starts_here && atomicAdd(n + blockIdx.x, 1u) == (unsigned)(e2 - (int)blockIdx.x);
+        cross[5] = starts_here && atomicAdd(n + block, 1u) == (unsigned)(e2 - (int)block);
       }
     }
     __syncthreads();
@@ -746,7 +816,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
 #pragma unroll
         for (int k = 0; k < N; ++k) ds[k] = add(ds[k], widen<A, V>(head + ((q << a.lg) + lane) * V, k));
       }
-      A* o = ds_part + (long long)blockIdx.x * 2 * dim + col;
+      A* o = ds_part + (long long)block * 2 * dim + col;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         narrow<A, V>(ds[k], o, k);
@@ -764,7 +834,7 @@ struct SumPlan {
 // long as they leave four blocks a SM.
 constexpr int kSms = 148;   // of a B200
 
-SumPlan sum_plan(long long n, long long rows, int nv) {
+SumPlan sum_plan(long long n, long long rows, int nv, long long row_bytes) {
   SumPlan p;
   p.lg = 0;
   while (p.lg < 5 && (1 << p.lg) < nv) ++p.lg;
@@ -773,8 +843,7 @@ SumPlan sum_plan(long long n, long long rows, int nv) {
   p.tile = 4;
   while ((p.tile < 32 && n * p.cols > 2LL * p.tile * ngrp * 4 * kSms) || n / ((long long)p.tile * ngrp) > 65536) p.tile *= 2;
   p.blocks = (int)((n + (long long)p.tile * ngrp - 1) / ((long long)p.tile * ngrp));
-  // rows of a warp: 32 short ones, fewer as they grow
-  p.fill = nv >= 128 ? 8 : nv >= 32 ? 16 : 32;
+  p.fill = row_bytes >= 32768 ? 1 : 32768 / (int)row_bytes < 32 ? 32768 / (int)row_bytes : 32;   // 32 KB a warp
   const long long warps = (rows + p.fill - 1) / p.fill, per = (long long)(kThreads / 32) * p.cols;
   p.fill_blocks = (int)((warps + per - 1) / per);
   return p;
@@ -790,7 +859,7 @@ ScatterLayout scatter_layout(long long rows, int dim, int dtype, long long n, in
   size_t blocks = 0, pieces = 0;
   for (int v = 1; v <= widest; v *= 2) {
     if (dim % v) break;
-    const SumPlan p = sum_plan(n, rows, dim / v);
+    const SumPlan p = sum_plan(n, rows, dim / v, (long long)dim * elem_size(dtype));
     if ((size_t)p.blocks > blocks) blocks = p.blocks;
     if ((size_t)p.blocks * p.cols > pieces) pieces = (size_t)p.blocks * p.cols;
   }
@@ -900,7 +969,7 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
     al.elements(ld_table);
   }
   const int vec = al.vec();
-  const SumPlan p = sum_plan(n, rows, dim / vec);
+  const SumPlan p = sum_plan(n, rows, dim / vec, (long long)dim * elem_size(dtype));
   SumArgs a = {};
   a.n = n;
   a.ld_g = ld_g;

@@ -1,0 +1,444 @@
+// features.cpp — the torch side of the node-feature operators: argument checks,
+// output and workspace allocation, autograd nodes, around the C entry points of
+// include/lanczos_b200.h.
+//
+// Compiled, where the rest of the package is bound with ctypes, because these
+// operators are called many times a step on small inputs: through ctypes and
+// Python autograd functions, layer norm forward and backward of 16 rows took
+// 125 us of host time.  gpu_eigsh/features.py has the documentation.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/extension.h>
+
+#include "../../../include/lanczos_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr int64_t kMaxRows = 2147483646;   // 2^31 - 2
+
+int code_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return LG_F32;
+    case at::kDouble: return LG_F64;
+    case at::kHalf: return LG_F16;
+    case at::kBFloat16: return LG_BF16;
+    default: return -1;
+  }
+}
+
+at::ScalarType acc_of(at::ScalarType t) { return t == at::kDouble ? at::kDouble : at::kFloat; }
+
+std::string name_of(at::ScalarType t) {   // as torch prints it
+  switch (t) {
+    case at::kFloat: return "torch.float32";
+    case at::kDouble: return "torch.float64";
+    case at::kHalf: return "torch.float16";
+    case at::kBFloat16: return "torch.bfloat16";
+    default: return c10::toString(t);
+  }
+}
+
+int check_features(const char* name, const Tensor& t) {
+  TORCH_CHECK_TYPE(t.is_cuda() && t.layout() == at::kStrided, name, " must be a CUDA tensor");
+  const int code = code_of(t.scalar_type());
+  TORCH_CHECK_TYPE(code >= 0, name, " must be float32, float64, float16 or bfloat16, got ", name_of(t.scalar_type()));
+  return code;
+}
+
+void check_device(const char* name, const Tensor& t, const char* other_name, const Tensor& other) {
+  TORCH_CHECK_VALUE(t.device() == other.device(), name, " is on ", t.device(), ", ", other_name, " on ", other.device());
+}
+
+// A failure of the library (RuntimeError, with the text of a LanczosError).
+void check_status(int rc) {
+  if (rc >= 0) return;
+  char text[1024] = {0};
+  lg_last_error(text, sizeof(text));
+  TORCH_CHECK(false, lg_status_string(rc), " (", rc, "): ", text);
+}
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// t as rows of `dim` values with unit stride along the row; copied only where the
+// strides do not allow that.
+struct Rows {
+  Tensor t;
+  int64_t ld;
+};
+Rows as_rows(const Tensor& t, int64_t dim) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, dim});
+  const int64_t n = r.size(0);
+  if ((dim > 1 && r.stride(1) != 1) || (n > 1 && r.stride(0) < dim)) r = r.contiguous();
+  return {r, n > 1 ? r.stride(0) : dim};
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+Tensor bytes(size_t n, const Tensor& like) {
+  return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
+}
+
+// An optional input of an autograd node: absent rather than undefined.  The node
+// counts only those that are there, so input k of those before it is
+// needs_input_grad(k).
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+Tensor plain(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+// Gradients that are not differentiable themselves: where a graph of the backward
+// pass is made, they lead to an error.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (auto& g : grads)
+    if (g.defined()) defined.push_back(g);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)defined.size());
+  variable_list inputs;
+  for (auto& g : defined) {
+    Tensor v = g.detach();
+    v.requires_grad_(true);
+    inputs.push_back(v);
+  }
+  variable_list outs = (*error)(std::move(inputs));
+  size_t k = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = outs[k++];
+  return grads;
+}
+
+// ---------------------------------------------------------------------------
+// Embedding lookup
+// ---------------------------------------------------------------------------
+struct LookupArgs {
+  int mode = LG_SCALE_NONE;
+  double value = 1.0;
+  bool has_pad = false;
+  int64_t pad = 0;
+};
+
+Tensor gather(const Tensor& table, const Tensor& column, const Tensor& ids, const LookupArgs& a) {
+  std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+  const int64_t rows = table.size(0), dim = table.size(1), n = ids.numel();
+  shape.push_back(dim);
+  Tensor out = at::empty(shape, table.options());
+  if (n) {
+    const c10::cuda::CUDAGuard guard(table.device());
+    const Rows t = as_rows(table, dim);
+    check_status(lg_rows_gather(rows, (int)dim, code_of(table.scalar_type()), t.t.data_ptr(), t.ld, n, ids.data_ptr(),
+                                ids.scalar_type() == at::kLong, a.mode, ptr(column), a.value, a.has_pad, a.pad,
+                                out.data_ptr(), stream_of(table)));
+  }
+  return out;
+}
+
+struct Lookup : public torch::autograd::Function<Lookup> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& scale, const Tensor& ids,
+                        int64_t mode, double value, bool has_pad, int64_t pad) {
+    const Tensor column = plain(scale);
+    ctx->save_for_backward({table, column, ids});
+    ctx->saved_data["mode"] = mode;
+    ctx->saved_data["value"] = value;
+    ctx->saved_data["has_pad"] = has_pad;
+    ctx->saved_data["pad"] = pad;
+    LookupArgs a;
+    a.mode = (int)mode;
+    a.value = value;
+    a.has_pad = has_pad;
+    a.pad = pad;
+    return gather(table, column, ids, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &table = saved[0], &column = saved[1], &ids = saved[2];
+    const int64_t rows = table.size(0), dim = table.size(1), n = ids.numel();
+    const int code = code_of(table.scalar_type());
+    const bool want_table = ctx->needs_input_grad(0), want_scale = column.defined() && ctx->needs_input_grad(1);
+    const c10::cuda::CUDAGuard guard(table.device());
+    Tensor d_table, d_scale;
+    if (want_table) d_table = n ? at::empty({rows, dim}, table.options()) : at::zeros({rows, dim}, table.options());
+    if (want_scale) d_scale = n ? at::empty({dim}, column.options()) : at::zeros({dim}, column.options());
+    if (n && (want_table || want_scale)) {
+      const Rows g = as_rows(grads[0], dim), t = as_rows(table, dim);
+      const size_t nb = lg_rows_scatter_workspace_bytes(rows, (int)dim, code, n, want_scale);
+      const Tensor ws = bytes(nb, table);
+      check_status(lg_rows_scatter(rows, (int)dim, code, t.t.data_ptr(), t.ld, n, ids.data_ptr(),
+                                   ids.scalar_type() == at::kLong, (int)ctx->saved_data["mode"].toInt(), ptr(column),
+                                   ctx->saved_data["value"].toDouble(), ctx->saved_data["has_pad"].toBool(),
+                                   ctx->saved_data["pad"].toInt(), g.t.data_ptr(), g.ld, ptr(d_table), ptr(d_scale),
+                                   ws.data_ptr(), nb, stream_of(table)));
+    }
+    return once({d_table, d_scale, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor embedding_lookup(const Tensor& table, const Tensor& ids, const std::optional<Tensor>& scale, double value,
+                        bool has_value, std::optional<int64_t> padding) {
+  check_features("table", table);
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "table must be (rows, dim), got shape ",
+                    table.sizes());
+  TORCH_CHECK_TYPE(ids.is_cuda() && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
+                   "ids must be an int32 or int64 CUDA tensor");
+  check_device("ids", ids, "table", table);
+  const int64_t dim = table.size(1);
+  TORCH_CHECK_VALUE(table.size(0) <= kMaxRows && ids.numel() <= kMaxRows && dim <= (1 << 20),
+                    "at most 2^31 - 2 rows and ids, and 2^20 columns");
+  LookupArgs a;
+  Tensor column;
+  if (scale.has_value()) {
+    const auto want = acc_of(table.scalar_type());
+    TORCH_CHECK_TYPE(scale->scalar_type() == want, "scale must be ", name_of(want), " for a ",
+                     name_of(table.scalar_type()), " table, got ", name_of(scale->scalar_type()));
+    TORCH_CHECK_VALUE(scale->dim() == 1 && scale->size(0) == dim, "scale must have shape (", dim, ",), got ", scale->sizes());
+    check_device("scale", *scale, "table", table);
+    a.mode = LG_SCALE_COLUMN;
+    column = scale->contiguous();
+  } else if (has_value) {
+    a.mode = LG_SCALE_VALUE;
+    a.value = value;
+  }
+  a.has_pad = padding.has_value();
+  a.pad = padding.value_or(0);
+  const Tensor at = ids.contiguous();
+  if (at::GradMode::is_enabled() && (table.requires_grad() || (column.defined() && column.requires_grad())))
+    return Lookup::apply(table, maybe(column), at, (int64_t)a.mode, a.value, a.has_pad, a.pad);
+  return gather(table, column, at, a);
+}
+
+// ---------------------------------------------------------------------------
+// Layer norm
+// ---------------------------------------------------------------------------
+int param_code(const Tensor& x, const Tensor& w, const Tensor& b) {
+  return code_of(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type());
+}
+
+Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, Tensor* stats) {
+  const int64_t dim = x.size(-1), rows = x.numel() / dim;
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty(x.sizes(), x.options());
+  const auto acc = acc_of(x.scalar_type());
+  char* mean = nullptr;
+  char* rstd = nullptr;
+  if (stats) {
+    *stats = at::empty({2, rows}, x.options().dtype(acc));
+    mean = static_cast<char*>(stats->data_ptr());
+    rstd = mean + rows * (acc == at::kDouble ? 8 : 4);
+  }
+  if (rows) {
+    const Rows t = as_rows(x, dim);
+    check_status(lg_layer_norm_forward(rows, (int)dim, code_of(x.scalar_type()), t.t.data_ptr(), t.ld, param_code(x, w, b),
+                                       ptr(w), ptr(b), eps, y.data_ptr(), mean, rstd, stream_of(x)));
+  }
+  return y;
+}
+
+struct LayerNorm : public torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
+                        const std::optional<Tensor>& bias, double eps) {
+    const Tensor w = plain(weight), b = plain(bias);
+    Tensor stats;
+    Tensor y = norm_forward(x, w, b, eps, &stats);
+    ctx->save_for_backward({x, w, stats});
+    ctx->saved_data["bias"] = b.defined();
+    ctx->saved_data["params"] = (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type());
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    const auto ptype = (at::ScalarType)ctx->saved_data["params"].toInt();
+    const int64_t dim = x.size(-1), rows = x.numel() / dim;
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto popt = x.options().dtype(ptype);
+    Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
+    if (w.defined() && ctx->needs_input_grad(1)) dw = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1))
+      db = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
+    if (rows && (dx.defined() || dw.defined() || db.defined())) {
+      const Rows t = as_rows(x, dim), g = as_rows(grads[0], dim);
+      const int code = code_of(x.scalar_type());
+      size_t nb = 0;
+      Tensor ws;
+      if (dw.defined() || db.defined()) {
+        nb = lg_layer_norm_workspace_bytes(rows, (int)dim, code);
+        ws = bytes(nb, x);
+      }
+      const char* mean = static_cast<const char*>(stats.data_ptr());
+      check_status(lg_layer_norm_backward(rows, (int)dim, code, t.t.data_ptr(), t.ld, g.t.data_ptr(), g.ld, code_of(ptype),
+                                          ptr(w), mean, mean + rows * stats.element_size(), ptr(dx), ptr(dw), ptr(db),
+                                          ptr(ws), nb, stream_of(x)));
+    }
+    return once({dx, dw, db, Tensor()});
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+  check_features("x", x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last dimension of at least 1, got shape ", x.sizes());
+  const int64_t dim = x.size(-1);
+  TORCH_CHECK_VALUE(x.numel() / dim <= kMaxRows && dim <= (1 << 24), "at most 2^31 - 2 rows and 2^24 columns");
+  TORCH_CHECK_VALUE(eps >= 0.0 && eps < std::numeric_limits<double>::infinity(),
+                    "eps must be finite and not negative, got ", eps);
+  const auto xt = x.scalar_type();
+  const bool half = xt == at::kHalf || xt == at::kBFloat16;
+  Tensor w, b;
+  for (int k = 0; k < 2; ++k) {
+    const auto& p = k ? bias : weight;
+    if (!p.has_value()) continue;
+    const char* name = k ? "bias" : "weight";
+    TORCH_CHECK_TYPE(p->is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK_TYPE(p->scalar_type() == xt || (half && p->scalar_type() == at::kFloat), name, " must be ", name_of(xt),
+                     half ? " or torch.float32" : "", ", got ", name_of(p->scalar_type()));
+    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == dim, name, " must have shape (", dim, ",), got ", p->sizes());
+    check_device(name, *p, "x", x);
+    (k ? b : w) = p->contiguous();
+  }
+  TORCH_CHECK_TYPE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
+                   "weight and bias must have the same type");
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
+    return LayerNorm::apply(x, maybe(w), maybe(b), eps);
+  return norm_forward(x, w, b, eps, nullptr);
+}
+
+// ---------------------------------------------------------------------------
+// Edge distances
+// ---------------------------------------------------------------------------
+// The lists of lg_edge_graph and those of its long vertices; shared by every call
+// (and every pending backward pass) that uses them.
+struct EdgeGraph : torch::CustomClassHolder {
+  int64_t n = 0, m = 0, nlong = 0, nchunks = 0;
+  Tensor ends, rowptr, lists;                                  // lists: other, then eid
+  Tensor long_row, long_first, chunk_row, chunk_first;
+  at::Device device = at::Device(at::kCPU);
+  void* built_on = nullptr;
+
+  // Makes the lists known to the current stream when it is not the one they were
+  // allocated on.
+  void use() const {
+    const auto cur = c10::cuda::getCurrentCUDAStream(device.index());
+    if (cur.stream() == built_on) return;
+    for (const Tensor* t : {&ends, &rowptr, &lists, &long_row, &long_first, &chunk_row, &chunk_first})
+      if (t->defined()) t->record_stream(cur);
+  }
+  const int* other() const { return lists.data_ptr<int>(); }
+  const int* eid() const { return lists.data_ptr<int>() + 2 * m; }
+};
+
+c10::intrusive_ptr<EdgeGraph> edge_graph(const Tensor& given, int64_t n) {
+  TORCH_CHECK_TYPE(given.is_cuda(), "idx must be a CUDA tensor");
+  TORCH_CHECK_TYPE(given.scalar_type() == at::kLong || given.scalar_type() == at::kInt,
+                   "idx must be int64 or int32, got ", name_of(given.scalar_type()));
+  TORCH_CHECK_VALUE(given.dim() == 2 && given.size(0) == 2, "idx must be (2, M), got shape ", given.sizes());
+  auto g = c10::make_intrusive<EdgeGraph>();
+  const int64_t m = given.size(1);
+  TORCH_CHECK_VALUE(n >= 1 && n <= kMaxRows && 2 * m <= kMaxRows,
+                    "n must be at least 1; at most 2^31 - 2 vertices and 2^30 - 1 edges");
+  g->n = n;
+  g->m = m;
+  g->device = given.device();
+  if (m == 0) return g;
+  const c10::cuda::CUDAGuard guard(given.device());
+  g->built_on = stream_of(given);
+  const Tensor idx = given.to(at::kLong).contiguous();
+  const auto i32 = idx.options().dtype(at::kInt);
+  g->ends = at::empty({2 * m}, i32);
+  g->rowptr = at::empty({n + 1}, i32);
+  g->lists = at::empty({4 * m}, i32);
+  Tensor found = at::empty({2}, i32);   // a bad index; the longest list
+  const size_t nb = lg_edge_graph_workspace_bytes(n, m);
+  const Tensor ws = bytes(nb, idx);
+  check_status(lg_edge_graph(n, m, reinterpret_cast<const long long*>(idx.data_ptr<int64_t>()), g->ends.data_ptr<int>(),
+                             g->rowptr.data_ptr<int>(), g->lists.data_ptr<int>(), g->lists.data_ptr<int>() + 2 * m,
+                             found.data_ptr<int>(), ws.data_ptr(), nb, stream_of(idx)));
+  const Tensor degree = g->rowptr.slice(0, 1) - g->rowptr.slice(0, 0, n);
+  found.slice(0, 1).copy_(degree.max().reshape({1}));
+  const Tensor host = found.cpu();
+  TORCH_CHECK_VALUE(host.data_ptr<int>()[0] == 0, "edge index out of range [0, n)");
+  if (host.data_ptr<int>()[1] <= LG_EDGE_CHUNK) return g;
+  // the vertices with long lists, and the chunks of their lists
+  const Tensor row = at::nonzero(degree > LG_EDGE_CHUNK).reshape({-1});
+  const Tensor count = at::floor_divide(degree.index_select(0, row).to(at::kLong) + (LG_EDGE_CHUNK - 1), LG_EDGE_CHUNK);
+  const Tensor first = at::cumsum(count, 0) - count;
+  const Tensor which = at::repeat_interleave(count);
+  const Tensor begin = g->rowptr.index_select(0, row).to(at::kLong).index_select(0, which) +
+                       (at::arange(which.numel(), row.options()) - first.index_select(0, which)) * LG_EDGE_CHUNK;
+  g->nlong = row.numel();
+  g->nchunks = which.numel();
+  g->long_row = row.to(at::kInt);
+  g->long_first = first.to(at::kInt);
+  g->chunk_row = row.index_select(0, which).to(at::kInt);
+  g->chunk_first = begin.to(at::kInt);
+  return g;
+}
+
+Tensor edge_forward(const Tensor& x, const EdgeGraph& g) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = at::empty({g.m}, x.options().dtype(acc_of(x.scalar_type())));
+  if (g.m) {
+    g.use();
+    const Rows t = as_rows(x, x.size(1));
+    check_status(lg_edge_sqdist(g.n, g.m, (int)x.size(1), code_of(x.scalar_type()), g.ends.data_ptr<int>(), t.t.data_ptr(),
+                                t.ld, out.data_ptr(), stream_of(x)));
+  }
+  return out;
+}
+
+struct EdgeDist : public torch::autograd::Function<EdgeDist> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::intrusive_ptr<EdgeGraph>& graph) {
+    ctx->save_for_backward({x});
+    ctx->saved_data["graph"] = graph;
+    return edge_forward(x, *graph);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor x = ctx->get_saved_variables()[0];
+    const auto graph = ctx->saved_data["graph"].toCustomClass<EdgeGraph>();
+    const EdgeGraph& e = *graph;
+    const int64_t dim = x.size(1);
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor dx = e.m ? at::empty({e.n, dim}, x.options()) : at::zeros({e.n, dim}, x.options());
+    if (e.m) {
+      e.use();
+      const Rows t = as_rows(x, dim);
+      const Tensor g = grads[0].contiguous();
+      const int code = code_of(x.scalar_type());
+      const size_t nb = lg_edge_sqdist_grad_workspace_bytes((int)e.nchunks, (int)dim, code);
+      const Tensor ws = nb ? bytes(nb, x) : Tensor();
+      auto list = [](const Tensor& l) { return l.defined() ? l.data_ptr<int>() : nullptr; };
+      check_status(lg_edge_sqdist_grad(e.n, e.m, (int)dim, code, e.rowptr.data_ptr<int>(), e.other(), e.eid(),
+                                       (int)e.nlong, list(e.long_row), list(e.long_first), (int)e.nchunks,
+                                       list(e.chunk_row), list(e.chunk_first), t.t.data_ptr(), t.ld, g.data_ptr(),
+                                       dx.data_ptr(), ptr(ws), nb, stream_of(x)));
+    }
+    return once({dx, Tensor()});
+  }
+};
+
+Tensor edge_sqdist(const Tensor& x, const c10::intrusive_ptr<EdgeGraph>& g) {
+  check_features("x", x);
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == g->n && x.size(1) >= 1 && x.size(1) <= (1 << 20), "x must be (", g->n,
+                    ", dim), got shape ", x.sizes());
+  TORCH_CHECK_VALUE(x.device() == g->device, "x is on ", x.device(), ", the edges on ", g->device);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return EdgeDist::apply(x, g);
+  return edge_forward(x, *g);
+}
+
+}  // namespace
+
+TORCH_LIBRARY(gpu_eigsh, m) { m.class_<EdgeGraph>("EdgeGraph"); }
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("embedding_lookup", &embedding_lookup, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+  py::class_<EdgeGraph, c10::intrusive_ptr<EdgeGraph>>(m, "EdgeGraph")
+      .def_readonly("n", &EdgeGraph::n)
+      .def_readonly("m", &EdgeGraph::m);
+  m.def("edge_graph", &edge_graph, py::call_guard<py::gil_scoped_release>());
+  m.def("edge_sqdist", &edge_sqdist, py::call_guard<py::gil_scoped_release>());
+}
