@@ -281,7 +281,7 @@ extern "C" int lg_edge_graph(long long n, long long m, const long long* idx, int
   if (e != cudaSuccess) return cuda_status(e, "lg_edge_graph");
   edge_check_kernel<<<wide_grid(2 * m), kThreads, 0, st>>>(n, m, idx, ends, bad);
   uint2* sorted = nullptr;
-  e = sort_ids(n, 2 * m, idx, 1, 0, 0, ws, nullptr, 0, &sorted, st);
+  e = sort_ids(n, 2 * m, idx, 1, 0, 0, ws, nullptr, 0, SideFill{nullptr, 0}, &sorted, st);
   if (e != cudaSuccess) return cuda_status(e, "lg_edge_graph");
   edge_lists_kernel<<<wide_grid(2 * m), kThreads, 0, st>>>(m, ends, sorted, other, eid);
   edge_rowptr_kernel<<<wide_grid(n + 1), kThreads, 0, st>>>(n, 2 * m, sorted, rowptr);

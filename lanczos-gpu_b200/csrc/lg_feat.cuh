@@ -236,9 +236,14 @@ inline int cuda_status(cudaError_t e, const char* where) {
 // those come last.  Equal keys keep the order of their positions.
 // ---------------------------------------------------------------------------
 size_t sort_ids_workspace(long long rows, long long n);
-// *sorted points into ws after the call.  `zero`: nzero words set to zero on the way.
+// *sorted points into ws after the call.  `zero`: nzero words set to zero on the
+// way; `fill`: bytes set to zero beside the sort.
+struct SideFill {
+  void* p;
+  size_t bytes;
+};
 cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, long long pad, int has_pad, void* ws,
-                     unsigned* zero, int nzero, uint2** sorted, cudaStream_t st);
+                     unsigned* zero, int nzero, SideFill fill, uint2** sorted, cudaStream_t st);
 
 // ---------------------------------------------------------------------------
 // out[c] = sum over r < nrows of part[r * ld + c] for c < dim; columns from
