@@ -563,6 +563,7 @@ struct SumArgs {
   int nv, lg, tile;          // vectors per row, lanes of a group, positions per group
   int blocks;                // blocks along the positions; those behind them set rows to zero
   int fill;                  // rows per warp of those
+  unsigned to_clear;         // the first rows, of which they clear the ones that no id names
   const uint2* sorted;
   unsigned* arrived;         // [column piece][block]: blocks of the run that starts there
   int mode;                  // scale
@@ -604,9 +605,9 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, unsigned v, int c, 
 template <typename T> __device__ __forceinline__ void fill_rows(const SumArgs& a, long long dim, long long block, T* dW) {
   const int lane = threadIdx.x & 31;
   const long long v0 = (block * (kThreads / 32) + (threadIdx.x >> 5)) * a.fill;
-  if (v0 >= a.rows) return;
+  if (v0 >= a.to_clear) return;
   const long long v = v0 + lane;
-  bool empty = lane < a.fill && v < a.rows;
+  bool empty = lane < a.fill && v < a.to_clear;
   if (empty) {
     unsigned lo = 0, hi = (unsigned)a.n;
     while (lo < hi) {
@@ -864,20 +865,19 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a, const T* __res
 }
 
 struct SumPlan {
-  int lg, cols, tile, blocks, fill, fill_blocks;
+  int lg, cols, tile, blocks, fill;
 };
 
 // Tiles of 4 to 32 positions (more where that would leave over 2^16 blocks): as
 // long as they leave four blocks a SM.
 constexpr int kSms = 148;   // of a B200
 
-// Bytes of rows written twice that clearing beside the sort is worth: what the SMs
-// that do not sort write in its time.  131072 x 2048 bf16 with 16384 ids (67 MB of
-// such rows): 146 us with the empty rows cleared by the sum's launch, 113 us with
-// all rows cleared beside the sort.
-constexpr size_t kSideFillMost = 96u << 20;
+// Bytes cleared beside the sort: about what the SMs that do not sort write in its
+// time.  131072 x 2048 bf16 with 16384 ids: 146 us with none, 130 us with all 537 MB
+// cleared there.
+constexpr long long kSideFillMost = 96LL << 20;
 
-SumPlan sum_plan(long long n, long long rows, int nv, long long row_bytes) {
+SumPlan sum_plan(long long n, int nv, long long row_bytes) {
   SumPlan p;
   p.lg = 0;
   while (p.lg < 5 && (1 << p.lg) < nv) ++p.lg;
@@ -887,8 +887,6 @@ SumPlan sum_plan(long long n, long long rows, int nv, long long row_bytes) {
   while ((p.tile < 32 && n * p.cols > 2LL * p.tile * ngrp * 4 * kSms) || n / ((long long)p.tile * ngrp) > 65536) p.tile *= 2;
   p.blocks = (int)((n + (long long)p.tile * ngrp - 1) / ((long long)p.tile * ngrp));
   p.fill = row_bytes >= 32768 ? 1 : 32768 / (int)row_bytes < 32 ? 32768 / (int)row_bytes : 32;   // 32 KB a warp
-  const long long warps = (rows + p.fill - 1) / p.fill, per = (long long)(kThreads / 32) * p.cols;
-  p.fill_blocks = (int)((warps + per - 1) / per);
   return p;
 }
 
@@ -902,7 +900,7 @@ ScatterLayout scatter_layout(long long rows, int dim, int dtype, long long n, in
   size_t blocks = 0, pieces = 0;
   for (int v = 1; v <= widest; v *= 2) {
     if (dim % v) break;
-    const SumPlan p = sum_plan(n, rows, dim / v, (long long)dim * elem_size(dtype));
+    const SumPlan p = sum_plan(n, dim / v, (long long)dim * elem_size(dtype));
     if ((size_t)p.blocks > blocks) blocks = p.blocks;
     if ((size_t)p.blocks * p.cols > pieces) pieces = (size_t)p.blocks * p.cols;
   }
@@ -1011,7 +1009,7 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
     al.elements(ld_table);
   }
   const int vec = al.vec();
-  const SumPlan p = sum_plan(n, rows, dim / vec, (long long)dim * elem_size(dtype));
+  const SumPlan p = sum_plan(n, dim / vec, (long long)dim * elem_size(dtype));
   SumArgs a = {};
   a.n = n;
   a.ld_g = ld_g;
@@ -1023,18 +1021,24 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
   a.want_ds = d_scale != nullptr;
   a.arrived = reinterpret_cast<unsigned*>(w + l.sort);
   uint2* sorted = nullptr;
-  // The sort keeps a few SMs busy for 10 to 30 us.  The others clear all of the
-  // gradient meanwhile, if the rows that ids name, which are then written twice, are
-  // few enough; else the sum's launch clears the rows that no id names.
-  const size_t row_bytes = (size_t)dim * elem_size(dtype);
+  // The sort keeps a few SMs busy for 10 to 30 us.  The others clear the last rows of
+  // the gradient meanwhile, of which those that ids name are then written twice; the
+  // sum's launch clears what is left of the rows that no id names.
+  const long long row_bytes = (long long)dim * elem_size(dtype);
+  long long cleared = 0;
+  if (d_table && n <= kClusterMost && n < rows) {
+    cleared = kSideFillMost / row_bytes;
+    if (cleared > rows) cleared = rows;
+  }
   SideFill side = {nullptr, 0};
-  if (d_table && n <= kClusterMost && (size_t)(n < rows ? n : rows) * row_bytes <= kSideFillMost)
-    side = {d_table, (size_t)rows * row_bytes};
+  if (cleared) side = {static_cast<char*>(d_table) + (rows - cleared) * row_bytes, (size_t)(cleared * row_bytes)};
+  a.to_clear = (unsigned)(d_table ? rows - cleared : 0);
   const cudaError_t e =
       sort_ids(rows, n, ids, ids64, padding, has_padding, w, a.arrived, p.blocks * p.cols, side, &sorted, st);
   if (e != cudaSuccess) return cuda_status(e, "lg_rows_scatter");
   a.sorted = sorted;
-  const int fill_blocks = d_table && !side.bytes ? p.fill_blocks : 0;
+  const long long per = (long long)p.fill * (kThreads / 32) * p.cols;
+  const int fill_blocks = (int)((a.to_clear + per - 1) / per);
   auto run = [&]() -> cudaError_t {
 #define LG_F(T, V)                                                                                                  \
   scatter_launch<T, V>(a, dim, static_cast<const T*>(g), static_cast<const T*>(table), static_cast<T*>(d_table), \
