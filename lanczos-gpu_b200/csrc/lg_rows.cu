@@ -343,7 +343,7 @@ __device__ __forceinline__ void side_fill(const SideFill& f, int me, int all) {
 
 template <int ITEMS>
 __global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(ClusterSortArgs c) {
-  extern __shared__ unsigned smem[];
+  extern __shared__ __align__(16) unsigned smem[];
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
   if ((int)blockIdx.x >= ctas) {   // not the first cluster
@@ -369,8 +369,9 @@ __global__ void __launch_bounds__(kClusterThreads, 1) sort_cluster_kernel(Cluste
       kv[i] = make_uint2(0, 0);
       if (p < a.n) kv[i] = pass ? __ldcg(a.in + p) : sort_pair(a, p);
     }
-    for (int i = threadIdx.x; i < kClusterWarps * digits; i += kClusterThreads) smem[i] = 0;
-    __syncthreads();
+    // a warp's counts are its own until the block adds them up
+    for (int i = lane * 4; i < digits; i += 128) *reinterpret_cast<uint4*>(own + i) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const bool in = p0 + 32 * i < a.n;
@@ -512,6 +513,7 @@ cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, lo
     c.buf[1] = buf[1];
     c.passes = (bits + 9) / 10;
     c.width = (bits + c.passes - 1) / c.passes;
+    if (c.width < 2) c.width = 2;   // a row of counts is a multiple of 16 bytes
     c.zero = zero;
     c.nzero = nzero;
     c.fill = fill;
