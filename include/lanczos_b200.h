@@ -533,12 +533,12 @@ int lg_layer_norm_backward(long long rows, int dim, int dtype, const void* x, lo
  * the other end; eid: the edge), the edges it begins before those it ends,
  * ascending.  *bad (device int) becomes 1 if an index is outside [0, n); the
  * lists are then not to be used.  2m < 2^31 - 1. */
-#define LG_EDGE_CHUNK 256
+#define LG_EDGE_CHUNK 128
 size_t lg_edge_graph_workspace_bytes(long long n, long long m);
 int lg_edge_graph(long long n, long long m, const long long* idx, int* ends, int* rowptr, int* other, int* eid,
                   int* bad, void* ws, size_t ws_bytes, void* stream);
 /* d2[e] = |x[begin_e, :] - x[end_e, :]|^2 in the accumulation type: the
- * x_edge_dists of the IMGP operator. */
+ * x_edge_dists of the IMGP operator.  Rows of x lie less than 4 GiB apart. */
 int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x, long long ld_x,
                    void* d2, void* stream);
 /* dx[v, :] = 2 sum over the edges e at v of g[e] (x[v, :] - x[other end, :]),

@@ -10,8 +10,11 @@
 // No atomics: the result does not change from run to run.  Vertices with more
 // than LG_EDGE_CHUNK edges are summed in chunks of that length, one group a
 // chunk, and the chunks' sums added in order, so a hub does not hold up the
-// rest.  Both directions are bound by the gathers of x rows (L2 as long as x
-// fits).
+// rest.
+//
+// Both directions are bound by the gathers of x rows from L2: by their latency, so
+// a group keeps several edges' rows in flight, and by the instructions around
+// them, so a lane takes two vectors of a row where the row has them.
 #include "lg_feat.cuh"
 
 #include "../../include/lanczos_b200.h"
@@ -61,142 +64,204 @@ __global__ void __launch_bounds__(kThreads) edge_rowptr_kernel(long long n, long
 }
 
 // ---------------------------------------------------------------------------
-// Distances: a group of 1 << lg lanes per edge
+// Distances: a group of 1 << lg lanes takes kEdges edges
 // ---------------------------------------------------------------------------
 struct EdgeArgs {
-  long long n, m, ld;
+  long long n, m;
+  unsigned stride;       // bytes from one row of x to the next
   int nv, lg;
 };
 
-template <typename T, int V>
+template <typename T> __device__ __forceinline__ const T* row_at(const T* x, int i, unsigned stride) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + (unsigned long long)(unsigned)i * stride);
+}
+
+constexpr int kEdges = 4;
+
+// K vectors a lane; LOOP: the row has more than K << lg.
+template <typename T, int V, int K, bool LOOP>
 __global__ void __launch_bounds__(kThreads) edge_dist_kernel(EdgeArgs a, const int* __restrict__ ends,
                                                              const T* __restrict__ x, Acc<T>* __restrict__ d2) {
   typedef Acc<T> A;
+  typedef Lane<T, V> L;
   const int lane = threadIdx.x & ((1 << a.lg) - 1);
   const int ngrp = kThreads >> a.lg;
-  const long long e = (long long)blockIdx.x * ngrp + (threadIdx.x >> a.lg);
-  A s = 0;
-  if (e < a.m) {
-    const T* xi = x + ends[e] * a.ld;
-    const T* xj = x + ends[a.m + e] * a.ld;
-    for (int c = lane; c < a.nv; c += 1 << a.lg) {
-      const Vec<T, V> u = load_vec<T, V>(xi + (long long)c * V), w = load_vec<T, V>(xj + (long long)c * V);
+  const long long e0 = (long long)blockIdx.x * ngrp * kEdges + (threadIdx.x >> a.lg);
+  const T *xi[kEdges], *xj[kEdges];
+  L s[kEdges];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const A d = to_acc(u.v[k]) - to_acc(w.v[k]);
-        s += d * d;
+  for (int u = 0; u < kEdges; ++u) {
+    const long long e = e0 + u * ngrp;
+    const bool in = e < a.m;
+    xi[u] = row_at(x, in ? ends[e] : 0, a.stride) + lane * V;
+    xj[u] = row_at(x, in ? ends[a.m + e] : 0, a.stride) + lane * V;
+    s[u] = spread<L>((A)0);
+  }
+  const L minus = spread<L>((A)-1);
+  for (int c = lane; c < (LOOP ? a.nv : lane + 1); c += K << a.lg) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (c + (k << a.lg) >= a.nv) break;
+      Vec<T, V> p[kEdges], q[kEdges];
+      const int at = (c - lane + (k << a.lg)) * V;
+#pragma unroll
+      for (int u = 0; u < kEdges; ++u) {
+        p[u] = load_vec<T, V>(xi[u] + at);
+        q[u] = load_vec<T, V>(xj[u] + at);
+      }
+#pragma unroll
+      for (int u = 0; u < kEdges; ++u) {
+#pragma unroll
+        for (int n = 0; n < lanes<V>; ++n) {
+          const L d = fma(widen<T, V>(q[u].v, n), minus, widen<T, V>(p[u].v, n));
+          s[u] = fma(d, d, s[u]);
+        }
       }
     }
   }
-  for (int o = 1 << a.lg >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0 && e < a.m) d2[e] = s;
+#pragma unroll
+  for (int u = 0; u < kEdges; ++u) {
+    A t = sum(s[u]);
+    for (int o = 1 << a.lg >> 1; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    const long long e = e0 + u * ngrp;
+    if (lane == 0 && e < a.m) d2[e] = t;
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Gradient: a group of lanes per vertex (or per chunk of a long list) and per
-// piece of 1 << lg vectors of the row (blockIdx.y)
+// piece of K << lg vectors of the row (blockIdx.y)
 // ---------------------------------------------------------------------------
-constexpr int kBatch = 4;
+struct GradArgs {
+  EdgeArgs e;
+  int nchunks;
+  const int *rowptr, *other, *eid, *chunk_row, *chunk_first;
+};
 
-template <typename T, int V>
-__device__ __forceinline__ void edge_row_sum(const EdgeArgs& a, long long v, int b, int e, int c,
-                                             const int* __restrict__ other, const int* __restrict__ eid,
-                                             const T* __restrict__ x, const Acc<T>* __restrict__ g, Acc<T>* acc) {
+// First the chunks, then the vertices.  A vertex row is written to dx, a chunk's
+// sum to part.  The indices of a batch of list entries are fetched while the rows
+// of the batch before are worked on.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kThreads) edge_grad_kernel(GradArgs a, const T* __restrict__ x,
+                                                             const Acc<T>* __restrict__ g, T* __restrict__ dx,
+                                                             Acc<T>* __restrict__ part) {
   typedef Acc<T> A;
-  const Vec<T, V> xv = load_vec<T, V>(x + v * a.ld + (long long)c * V);
-  for (int q = b; q < e; q += kBatch) {
-    int o[kBatch];
-    A w[kBatch];
-    Vec<T, V> y[kBatch];
+  typedef Lane<T, V> L;
+  constexpr int N = lanes<V>, B = 4;
+  const int lg = a.e.lg, lane = threadIdx.x & ((1 << lg) - 1);
+  const long long unit = (long long)blockIdx.x * (kThreads >> lg) + (threadIdx.x >> lg);
+  const bool chunk = unit < a.nchunks;
+  if (unit >= a.nchunks + a.e.n) return;
+  const long long v = chunk ? a.chunk_row[unit] : unit - a.nchunks;
+  int b = a.rowptr[v], e = a.rowptr[v + 1];
+  if (chunk) {
+    b = a.chunk_first[unit];
+    if (e - b > LG_EDGE_CHUNK) e = b + LG_EDGE_CHUNK;
+  } else if (e - b > LG_EDGE_CHUNK) {
+    return;   // summed by chunks
+  }
+  int at[K];
+  bool on[K];
+  Vec<T, V> own[K];
+  L acc[K][N];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int p = q + u < e ? q + u : e - 1;
-      o[u] = other[p];
-      w[u] = g[eid[p]];
+  for (int k = 0; k < K; ++k) {
+    const int c = (blockIdx.y * K + k) * (1 << lg) + lane;
+    on[k] = c < a.e.nv;
+    at[k] = on[k] ? c * V : 0;
+    own[k] = load_vec<T, V>(row_at(x, (int)v, a.e.stride) + at[k]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[k][n] = spread<L>((A)0);
+  }
+  const L minus = spread<L>((A)-1);
+  int next[B];
+  A w_next[B];
+#pragma unroll
+  for (int u = 0; u < B; ++u) {
+    next[u] = b + u < e ? a.other[b + u] : (int)v;
+    w_next[u] = b + u < e ? g[a.eid[b + u]] : (A)0;
+  }
+  for (int q = b; q < e; q += B) {
+    Vec<T, V> y[B][K];
+    A w[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const T* r = row_at(x, next[u], a.e.stride);
+#pragma unroll
+      for (int k = 0; k < K; ++k) y[u][k] = load_vec<T, V>(r + at[k]);
+      w[u] = w_next[u];
+    }
+    const int p = q + B;
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      next[u] = p + u < e ? a.other[p + u] : (int)v;
+      w_next[u] = p + u < e ? g[a.eid[p + u]] : (A)0;
     }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) y[u] = load_vec<T, V>(x + o[u] * a.ld + (long long)c * V);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
+    for (int u = 0; u < B; ++u) {
       if (q + u < e) {
+        const L f = spread<L>(w[u]);
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += w[u] * (to_acc(xv.v[k]) - to_acc(y[u].v[k]));
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            acc[k][n] = fma(f, fma(widen<T, V>(y[u][k].v, n), minus, widen<T, V>(own[k].v, n)), acc[k][n]);
       }
+    }
+  }
+  const long long dim = (long long)a.e.nv * V;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (!on[k]) continue;
+    if (chunk) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) narrow<A, V>(acc[k][n], part + unit * dim + at[k], n);
+    } else {
+      Vec<T, V> o;
+      const L two = spread<L>((A)2);
+#pragma unroll
+      for (int n = 0; n < N; ++n) narrow<T, V>(mul(acc[k][n], two), o.v, n);
+      store_vec<T, V>(dx + v * dim + at[k], o);
+    }
   }
 }
 
-template <typename T, int V> __device__ __forceinline__ void edge_store(T* p, const Acc<T>* acc) {
-  Vec<T, V> o;
-#pragma unroll
-  for (int k = 0; k < V; ++k) o.v[k] = from_acc<T>((Acc<T>)2 * acc[k]);
-  store_vec<T, V>(p, o);
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) edge_grad_kernel(EdgeArgs a, const int* __restrict__ rowptr,
-                                                             const int* __restrict__ other, const int* __restrict__ eid,
-                                                             const T* __restrict__ x, const Acc<T>* __restrict__ g,
-                                                             T* __restrict__ dx) {
-  const int lane = threadIdx.x & ((1 << a.lg) - 1);
-  const int ngrp = kThreads >> a.lg;
-  const long long v = (long long)blockIdx.x * ngrp + (threadIdx.x >> a.lg);
-  const int c = (blockIdx.y << a.lg) + lane;
-  if (v >= a.n || c >= a.nv) return;
-  const int b = rowptr[v], e = rowptr[v + 1];
-  if (e - b > LG_EDGE_CHUNK) return;   // summed by chunks
-  Acc<T> acc[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = 0;
-  edge_row_sum<T, V>(a, v, b, e, c, other, eid, x, g, acc);
-  edge_store<T, V>(dx + v * a.nv * V + (long long)c * V, acc);
-}
-
-// Chunks of the long lists: chunk_row names the vertex, chunk_first the first
-// position of its list entry in other / eid.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) edge_chunk_kernel(EdgeArgs a, int nchunks, const int* __restrict__ rowptr,
-                                                              const int* __restrict__ other, const int* __restrict__ eid,
-                                                              const int* __restrict__ chunk_row,
-                                                              const int* __restrict__ chunk_first,
-                                                              const T* __restrict__ x, const Acc<T>* __restrict__ g,
-                                                              Acc<T>* __restrict__ part) {
-  const int lane = threadIdx.x & ((1 << a.lg) - 1);
-  const int ngrp = kThreads >> a.lg;
-  const long long q = (long long)blockIdx.x * ngrp + (threadIdx.x >> a.lg);
-  const int c = (blockIdx.y << a.lg) + lane;
-  if (q >= nchunks || c >= a.nv) return;
-  const int v = chunk_row[q], b = chunk_first[q];
-  const int end = rowptr[v + 1], e = end - b > LG_EDGE_CHUNK ? b + LG_EDGE_CHUNK : end;
-  Acc<T> acc[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = 0;
-  edge_row_sum<T, V>(a, v, b, e, c, other, eid, x, g, acc);
-  Acc<T>* o = part + q * a.nv * V + (long long)c * V;
-#pragma unroll
-  for (int k = 0; k < V; ++k) o[k] = acc[k];
-}
-
-// One block row per long vertex: its first chunk is long_first[r], the chunks
-// follow one another.
+// The long vertices: a block adds 32 columns of a vertex's chunks (from
+// long_first[r] on, one after the other), eight rows of threads taking every
+// eighth chunk.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) edge_long_kernel(int dim, const int* __restrict__ rowptr,
                                                              const int* __restrict__ long_row,
-                                                             const int* __restrict__ long_first,
-                                                             const Acc<T>* __restrict__ part, T* __restrict__ dx) {
-  const long long v = long_row[blockIdx.x];
-  const long long q0 = long_first[blockIdx.x];
+                                                             const int* __restrict__ long_first, const Acc<T>* part,
+                                                             T* __restrict__ dx) {
+  __shared__ Acc<T> red[kThreads / 32][33];
+  griddep_wait();
+  const long long v = long_row[blockIdx.x], q0 = long_first[blockIdx.x];
   const int count = (rowptr[v + 1] - rowptr[v] + LG_EDGE_CHUNK - 1) / LG_EDGE_CHUNK;
-  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < dim; c += gridDim.y * blockDim.x) {
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  for (int c0 = blockIdx.y * 32; c0 < dim; c0 += gridDim.y * 32) {
+    const int c = c0 + lane;
     Acc<T> s = 0;
-#pragma unroll 8
-    for (int k = 0; k < count; ++k) s += part[(q0 + k) * dim + c];
-    dx[v * dim + c] = from_acc<T>((Acc<T>)2 * s);
+    if (c < dim) {
+#pragma unroll 4
+      for (int k = grp; k < count; k += kThreads / 32) s += part[(q0 + k) * dim + c];
+    }
+    __syncthreads();
+    red[grp][lane] = s;
+    __syncthreads();
+    if (grp == 0 && c < dim) {
+      Acc<T> t = 0;
+#pragma unroll
+      for (int k = 0; k < kThreads / 32; ++k) t += red[k][lane];
+      dx[v * dim + c] = from_acc<T>((Acc<T>)2 * t);
+    }
   }
 }
 
+// Lanes of a group, each with up to two vectors of the row.
 int group_log(int nv) {
   int l = 0;
-  while (l < 5 && (1 << l) < nv) ++l;
+  while (l < 5 && (2 << l) < nv) ++l;
   return l;
 }
 
@@ -204,44 +269,49 @@ template <typename T, int V>
 cudaError_t edge_dist(EdgeArgs a, int dim, const int* ends, const T* x, void* d2, cudaStream_t st) {
   a.nv = dim / V;
   a.lg = group_log(a.nv);
-  const int ngrp = kThreads >> a.lg;
-  edge_dist_kernel<T, V><<<(unsigned)((a.m + ngrp - 1) / ngrp), kThreads, 0, st>>>(a, ends, x, static_cast<Acc<T>*>(d2));
+  const int per = (kThreads >> a.lg) * kEdges;
+  const unsigned grid = (unsigned)((a.m + per - 1) / per);
+  Acc<T>* out = static_cast<Acc<T>*>(d2);
+  if (a.nv > 64) edge_dist_kernel<T, V, 2, true><<<grid, kThreads, 0, st>>>(a, ends, x, out);
+  else if (a.nv > 1) edge_dist_kernel<T, V, 2, false><<<grid, kThreads, 0, st>>>(a, ends, x, out);
+  else edge_dist_kernel<T, V, 1, false><<<grid, kThreads, 0, st>>>(a, ends, x, out);
   return cudaGetLastError();
 }
 
 struct LongLists {
-  int nlong, nchunks;
-  const int *row, *first, *chunk_row, *chunk_first;
+  int nlong;
+  const int *row, *first;
 };
 
 template <typename T, int V>
-cudaError_t edge_grad(EdgeArgs a, int dim, const int* rowptr, const int* other, const int* eid, const T* x,
-                      const void* g, T* dx, const LongLists& l, void* ws, cudaStream_t st) {
+cudaError_t edge_grad(GradArgs a, int dim, const T* x, const void* g, T* dx, const LongLists& l, void* ws,
+                      cudaStream_t st) {
   typedef Acc<T> A;
-  a.nv = dim / V;
-  a.lg = group_log(a.nv);
-  const int ngrp = kThreads >> a.lg;
-  const unsigned cols = (unsigned)((a.nv + (1 << a.lg) - 1) >> a.lg);
+  a.e.nv = dim / V;
+  a.e.lg = group_log(a.e.nv);
+  const int ngrp = kThreads >> a.e.lg;
+  const unsigned cols = (unsigned)((a.e.nv + (2 << a.e.lg) - 1) / (2 << a.e.lg));
+  A* part = static_cast<A*>(ws);
+  const dim3 grid((unsigned)((a.e.n + a.nchunks + ngrp - 1) / ngrp), cols);
   const A* gv = static_cast<const A*>(g);
-  edge_grad_kernel<T, V><<<dim3((unsigned)((a.n + ngrp - 1) / ngrp), cols), kThreads, 0, st>>>(a, rowptr, other, eid, x,
-                                                                                              gv, dx);
-  if (l.nlong > 0) {
-    A* part = static_cast<A*>(ws);
-    edge_chunk_kernel<T, V><<<dim3((unsigned)((l.nchunks + ngrp - 1) / ngrp), cols), kThreads, 0, st>>>(
-        a, l.nchunks, rowptr, other, eid, l.chunk_row, l.chunk_first, x, gv, part);
-    const unsigned pieces = (unsigned)((dim + kThreads - 1) / kThreads);
-    edge_long_kernel<T><<<dim3((unsigned)l.nlong, pieces < 65535u ? pieces : 65535u), kThreads, 0, st>>>(
-        dim, rowptr, l.row, l.first, part, dx);
+  if (a.e.nv > 1) edge_grad_kernel<T, V, 2><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  else edge_grad_kernel<T, V, 1><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && l.nlong > 0) {
+    const unsigned pieces = (unsigned)((dim + 31) / 32);
+    e = launch_pdl(edge_long_kernel<T>, dim3((unsigned)l.nlong, pieces < 65535u ? pieces : 65535u), dim3(kThreads), 0, st,
+                   dim, a.rowptr, l.row, l.first, part, dx);
   }
-  return cudaGetLastError();
+  return e;
 }
 
 bool edge_sizes_ok(long long n, long long m) {
   return n >= 1 && n < 2147483647LL && m >= 1 && 2 * m < 2147483647LL;
 }
 
-bool edge_args_ok(long long n, long long m, int dim, int dtype) {
-  return edge_sizes_ok(n, m) && dim >= 1 && dim <= (1 << 20) && elem_size(dtype);
+bool edge_args_ok(long long n, long long m, int dim, int dtype, long long ld) {
+  return edge_sizes_ok(n, m) && dim >= 1 && dim <= (1 << 20) && elem_size(dtype) && ld >= dim &&
+         ld * elem_size(dtype) < (1LL << 32);
 }
 
 int wide_grid(long long n) {
@@ -290,12 +360,12 @@ extern "C" int lg_edge_graph(long long n, long long m, const long long* idx, int
 
 extern "C" int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x,
                               long long ld_x, void* d2, void* stream) {
-  if (!edge_args_ok(n, m, dim, dtype) || !ends || !x || ld_x < dim || !d2)
+  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !ends || !x || !d2)
     return bad_args("lg_edge_sqdist: invalid arguments");
   EdgeArgs a = {};
   a.n = n;
   a.m = m;
-  a.ld = ld_x;
+  a.stride = (unsigned)(ld_x * elem_size(dtype));
   Align al(elem_size(dtype));
   al.address(x);
   al.elements(ld_x);
@@ -318,26 +388,31 @@ extern "C" int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype,
                                    const int* eid, int nlong, const int* long_row, const int* long_first, int nchunks,
                                    const int* chunk_row, const int* chunk_first, const void* x, long long ld_x,
                                    const void* g, void* dx, void* ws, size_t ws_bytes, void* stream) {
-  if (!edge_args_ok(n, m, dim, dtype) || !rowptr || !other || !eid || !x || ld_x < dim || !g || !dx || nlong < 0 ||
+  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !rowptr || !other || !eid || !x || !g || !dx || nlong < 0 ||
       nchunks < nlong ||
       (nlong > 0 && (!long_row || !long_first || !chunk_row || !chunk_first || !ws ||
                      ws_bytes < lg_edge_sqdist_grad_workspace_bytes(nchunks, dim, dtype))))
     return bad_args("lg_edge_sqdist_grad: invalid arguments");
-  EdgeArgs a = {};
-  a.n = n;
-  a.m = m;
-  a.ld = ld_x;
+  GradArgs a = {};
+  a.e.n = n;
+  a.e.m = m;
+  a.e.stride = (unsigned)(ld_x * elem_size(dtype));
+  a.nchunks = nlong > 0 ? nchunks : 0;
+  a.rowptr = rowptr;
+  a.other = other;
+  a.eid = eid;
+  a.chunk_row = chunk_row;
+  a.chunk_first = chunk_first;
   Align al(elem_size(dtype));
   al.address(x);
   al.address(dx);
   al.elements(ld_x);
   al.elements(dim);
   const int vec = al.vec();
-  const LongLists l = {nlong, nchunks, long_row, long_first, chunk_row, chunk_first};
+  const LongLists l = {nlong, long_row, long_first};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&]() -> cudaError_t {
-#define LG_F(T, V) \
-  edge_grad<T, V>(a, dim, rowptr, other, eid, static_cast<const T*>(x), g, static_cast<T*>(dx), l, ws, st)
+#define LG_F(T, V) edge_grad<T, V>(a, dim, static_cast<const T*>(x), g, static_cast<T*>(dx), l, ws, st)
     LG_EDGE_DISPATCH(LG_F)
 #undef LG_F
   };

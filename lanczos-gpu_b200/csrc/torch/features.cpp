@@ -74,7 +74,10 @@ struct Rows {
 Rows as_rows(const Tensor& t, int64_t dim) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, dim});
   const int64_t n = r.size(0);
-  if ((dim > 1 && r.stride(1) != 1) || (n > 1 && r.stride(0) < dim)) r = r.contiguous();
+  // (and rows 4 GiB apart and more, which the edge kernels do not address)
+  if ((dim > 1 && r.stride(1) != 1) ||
+      (n > 1 && (r.stride(0) < dim || r.stride(0) >= (int64_t)(1LL << 32) / (int64_t)r.element_size())))
+    r = r.contiguous();
   return {r, n > 1 ? r.stride(0) : dim};
 }
 

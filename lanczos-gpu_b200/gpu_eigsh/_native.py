@@ -88,7 +88,7 @@ LG_F64 = 1
 LG_F16 = 2
 LG_BF16 = 3
 LG_SCALE_NONE, LG_SCALE_VALUE, LG_SCALE_COLUMN = 0, 1, 2
-LG_EDGE_CHUNK = 256
+LG_EDGE_CHUNK = 128
 FUNCS = {"log": 0, "exp": 1, "sqrt": 2, "inv": 3}
 
 
