@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) edge_grad_kernel(GradArgs a, const T
                                                              Acc<T>* __restrict__ part) {
   typedef Acc<T> A;
   typedef Lane<T, V> L;
-  constexpr int N = lanes<V>, B = 4;
+  constexpr int N = lanes<V>, B = 4;   // list entries in flight
   const int lg = a.e.lg, lane = threadIdx.x & ((1 << lg) - 1);
   const long long unit = (long long)blockIdx.x * (kThreads >> lg) + (threadIdx.x >> lg);
   const bool chunk = unit < a.nchunks;
@@ -174,28 +174,29 @@ __global__ void __launch_bounds__(kThreads) edge_grad_kernel(GradArgs a, const T
     for (int n = 0; n < N; ++n) acc[k][n] = spread<L>((A)0);
   }
   const L minus = spread<L>((A)-1);
-  int next[B];
-  A w_next[B];
+  int next[B], edge[B];
 #pragma unroll
   for (int u = 0; u < B; ++u) {
     next[u] = b + u < e ? a.other[b + u] : (int)v;
-    w_next[u] = b + u < e ? g[a.eid[b + u]] : (A)0;
+    edge[u] = b + u < e ? a.eid[b + u] : -1;
   }
   for (int q = b; q < e; q += B) {
     Vec<T, V> y[B][K];
     A w[B];
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      const T* r = row_at(x, next[u], a.e.stride);
+      if (edge[u] >= 0) {
+        const T* r = row_at(x, next[u], a.e.stride);
+        w[u] = g[edge[u]];
 #pragma unroll
-      for (int k = 0; k < K; ++k) y[u][k] = load_vec<T, V>(r + at[k]);
-      w[u] = w_next[u];
+        for (int k = 0; k < K; ++k) y[u][k] = load_vec<T, V>(r + at[k]);
+      }
     }
     const int p = q + B;
 #pragma unroll
     for (int u = 0; u < B; ++u) {
       next[u] = p + u < e ? a.other[p + u] : (int)v;
-      w_next[u] = p + u < e ? g[a.eid[p + u]] : (A)0;
+      edge[u] = p + u < e ? a.eid[p + u] : -1;
     }
 #pragma unroll
     for (int u = 0; u < B; ++u) {
