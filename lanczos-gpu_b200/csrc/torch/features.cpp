@@ -5,11 +5,15 @@
 // Compiled, where the rest of the package is bound with ctypes, because these
 // operators are called many times a step on small inputs: through ctypes and
 // Python autograd functions, layer norm forward and backward of 16 rows took
-// 125 us of host time.  gpu_eigsh/features.py has the documentation.
+// 125 us of host time.  The autograd nodes are plain Nodes with saved variables,
+// which cost a few us less a pass than torch::autograd::Function's.
+// gpu_eigsh/features.py has the documentation.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include "../../../include/lanczos_b200.h"
@@ -17,7 +21,8 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 constexpr int64_t kMaxRows = 2147483646;   // 2^31 - 2
@@ -87,11 +92,14 @@ Tensor bytes(size_t n, const Tensor& like) {
   return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
 }
 
-// An optional input of an autograd node: absent rather than undefined.  The node
-// counts only those that are there, so input k of those before it is
-// needs_input_grad(k).
-std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
-Tensor plain(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A node over the inputs; it has a gradient for each, also for undefined ones.
+template <typename N, typename... Ts> std::shared_ptr<N> node_of(const Ts&... inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
+}
 
 // Gradients that are not differentiable themselves: where a graph of the backward
 // pass is made, they lead to an error.
@@ -140,43 +148,35 @@ Tensor gather(const Tensor& table, const Tensor& column, const Tensor& ids, cons
   return out;
 }
 
-struct Lookup : public torch::autograd::Function<Lookup> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& table, const std::optional<Tensor>& scale, const Tensor& ids,
-                        int64_t mode, double value, bool has_pad, int64_t pad) {
-    const Tensor column = plain(scale);
-    ctx->save_for_backward({table, column, ids});
-    ctx->saved_data["mode"] = mode;
-    ctx->saved_data["value"] = value;
-    ctx->saved_data["has_pad"] = has_pad;
-    ctx->saved_data["pad"] = pad;
-    LookupArgs a;
-    a.mode = (int)mode;
-    a.value = value;
-    a.has_pad = has_pad;
-    a.pad = pad;
-    return gather(table, column, ids, a);
+struct LookupBackward : public Node {
+  SavedVariable table, column, ids;
+  LookupArgs args;
+
+  std::string name() const override { return "EmbeddingLookupBackward"; }
+  void release_variables() override {
+    table.reset_data();
+    column.reset_data();
+    ids.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list saved = ctx->get_saved_variables();
-    const Tensor &table = saved[0], &column = saved[1], &ids = saved[2];
-    const int64_t rows = table.size(0), dim = table.size(1), n = ids.numel();
-    const int code = code_of(table.scalar_type());
-    const bool want_table = ctx->needs_input_grad(0), want_scale = column.defined() && ctx->needs_input_grad(1);
-    const c10::cuda::CUDAGuard guard(table.device());
-    Tensor d_table, d_scale;
-    if (want_table) d_table = n ? at::empty({rows, dim}, table.options()) : at::zeros({rows, dim}, table.options());
-    if (want_scale) d_scale = n ? at::empty({dim}, column.options()) : at::zeros({dim}, column.options());
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    if (!grads[0].defined()) return out;
+    const Tensor w = table.unpack(), c = column.unpack(), at = ids.unpack();
+    const int64_t rows = w.size(0), dim = w.size(1), n = at.numel();
+    const int code = code_of(w.scalar_type());
+    const bool want_table = task_should_compute_output(0), want_scale = c.defined() && task_should_compute_output(1);
+    const c10::cuda::CUDAGuard guard(w.device());
+    if (want_table) out[0] = n ? at::empty({rows, dim}, w.options()) : at::zeros({rows, dim}, w.options());
+    if (want_scale) out[1] = n ? at::empty({dim}, c.options()) : at::zeros({dim}, c.options());
     if (n && (want_table || want_scale)) {
-      const Rows g = as_rows(grads[0], dim), t = as_rows(table, dim);
+      const Rows g = as_rows(grads[0], dim), t = as_rows(w, dim);
       const size_t nb = lg_rows_scatter_workspace_bytes(rows, (int)dim, code, n, want_scale);
-      const Tensor ws = bytes(nb, table);
-      check_status(lg_rows_scatter(rows, (int)dim, code, t.t.data_ptr(), t.ld, n, ids.data_ptr(),
-                                   ids.scalar_type() == at::kLong, (int)ctx->saved_data["mode"].toInt(), ptr(column),
-                                   ctx->saved_data["value"].toDouble(), ctx->saved_data["has_pad"].toBool(),
-                                   ctx->saved_data["pad"].toInt(), g.t.data_ptr(), g.ld, ptr(d_table), ptr(d_scale),
-                                   ws.data_ptr(), nb, stream_of(table)));
+      const Tensor ws = bytes(nb, w);
+      check_status(lg_rows_scatter(rows, (int)dim, code, t.t.data_ptr(), t.ld, n, at.data_ptr(),
+                                   at.scalar_type() == at::kLong, args.mode, ptr(c), args.value, args.has_pad, args.pad,
+                                   g.t.data_ptr(), g.ld, ptr(out[0]), ptr(out[1]), ws.data_ptr(), nb, stream_of(w)));
     }
-    return once({d_table, d_scale, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    return once(std::move(out));
   }
 };
 
@@ -208,9 +208,21 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, const std::optio
   a.has_pad = padding.has_value();
   a.pad = padding.value_or(0);
   const Tensor at = ids.contiguous();
-  if (at::GradMode::is_enabled() && (table.requires_grad() || (column.defined() && column.requires_grad())))
-    return Lookup::apply(table, maybe(column), at, (int64_t)a.mode, a.value, a.has_pad, a.pad);
-  return gather(table, column, at, a);
+  const bool differentiate = at::GradMode::is_enabled() && (wants_grad(table) || wants_grad(column));
+  Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    out = gather(table, column, at, a);
+  }
+  if (differentiate) {
+    auto node = node_of<LookupBackward>(table, column);
+    node->table = SavedVariable(table, false);
+    node->column = SavedVariable(column, false);
+    node->ids = SavedVariable(at, false);
+    node->args = a;
+    torch::autograd::set_history(out, node);
+  }
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -240,44 +252,42 @@ Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double ep
   return y;
 }
 
-struct LayerNorm : public torch::autograd::Function<LayerNorm> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
-                        const std::optional<Tensor>& bias, double eps) {
-    const Tensor w = plain(weight), b = plain(bias);
-    Tensor stats;
-    Tensor y = norm_forward(x, w, b, eps, &stats);
-    ctx->save_for_backward({x, w, stats});
-    ctx->saved_data["bias"] = b.defined();
-    ctx->saved_data["params"] = (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type());
-    return y;
+struct LayerNormBackward : public Node {
+  SavedVariable x, weight, stats;
+  at::ScalarType params = at::kFloat;
+
+  std::string name() const override { return "LayerNormBackward"; }
+  void release_variables() override {
+    x.reset_data();
+    weight.reset_data();
+    stats.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
-    const auto ptype = (at::ScalarType)ctx->saved_data["params"].toInt();
-    const int64_t dim = x.size(-1), rows = x.numel() / dim;
-    const c10::cuda::CUDAGuard guard(x.device());
-    const auto popt = x.options().dtype(ptype);
-    Tensor dx, dw, db;
-    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
-    if (w.defined() && ctx->needs_input_grad(1)) dw = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
-    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.defined() ? 2 : 1))
-      db = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const Tensor v = x.unpack(), w = weight.unpack(), s = stats.unpack();
+    const int64_t dim = v.size(-1), rows = v.numel() / dim;
+    const c10::cuda::CUDAGuard guard(v.device());
+    const auto popt = v.options().dtype(params);
+    Tensor &dx = out[0], &dw = out[1], &db = out[2];
+    if (task_should_compute_output(0)) dx = at::empty(v.sizes(), v.options());
+    if (task_should_compute_output(1)) dw = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
+    if (task_should_compute_output(2)) db = rows ? at::empty({dim}, popt) : at::zeros({dim}, popt);
     if (rows && (dx.defined() || dw.defined() || db.defined())) {
-      const Rows t = as_rows(x, dim), g = as_rows(grads[0], dim);
-      const int code = code_of(x.scalar_type());
+      const Rows t = as_rows(v, dim), g = as_rows(grads[0], dim);
+      const int code = code_of(v.scalar_type());
       size_t nb = 0;
       Tensor ws;
       if (dw.defined() || db.defined()) {
         nb = lg_layer_norm_workspace_bytes(rows, (int)dim, code);
-        ws = bytes(nb, x);
+        ws = bytes(nb, v);
       }
-      const char* mean = static_cast<const char*>(stats.data_ptr());
-      check_status(lg_layer_norm_backward(rows, (int)dim, code, t.t.data_ptr(), t.ld, g.t.data_ptr(), g.ld, code_of(ptype),
-                                          ptr(w), mean, mean + rows * stats.element_size(), ptr(dx), ptr(dw), ptr(db),
-                                          ptr(ws), nb, stream_of(x)));
+      const char* mean = static_cast<const char*>(s.data_ptr());
+      check_status(lg_layer_norm_backward(rows, (int)dim, code, t.t.data_ptr(), t.ld, g.t.data_ptr(), g.ld, code_of(params),
+                                          ptr(w), mean, mean + rows * s.element_size(), ptr(dx), ptr(dw), ptr(db), ptr(ws),
+                                          nb, stream_of(v)));
     }
-    return once({dx, dw, db, Tensor()});
+    return once(std::move(out));
   }
 };
 
@@ -304,10 +314,21 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   }
   TORCH_CHECK_TYPE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
                    "weight and bias must have the same type");
-  if (at::GradMode::is_enabled() &&
-      (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
-    return LayerNorm::apply(x, maybe(w), maybe(b), eps);
-  return norm_forward(x, w, b, eps, nullptr);
+  const bool differentiate = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b));
+  Tensor out, stats;
+  {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    out = norm_forward(x, w, b, eps, differentiate ? &stats : nullptr);
+  }
+  if (differentiate) {
+    auto node = node_of<LayerNormBackward>(x, w, b);
+    node->x = SavedVariable(x, false);
+    node->weight = SavedVariable(w, false);
+    node->stats = SavedVariable(stats, false);
+    node->params = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : xt;
+    torch::autograd::set_history(out, node);
+  }
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -393,33 +414,33 @@ Tensor edge_forward(const Tensor& x, const EdgeGraph& g) {
   return out;
 }
 
-struct EdgeDist : public torch::autograd::Function<EdgeDist> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::intrusive_ptr<EdgeGraph>& graph) {
-    ctx->save_for_backward({x});
-    ctx->saved_data["graph"] = graph;
-    return edge_forward(x, *graph);
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor x = ctx->get_saved_variables()[0];
-    const auto graph = ctx->saved_data["graph"].toCustomClass<EdgeGraph>();
+struct EdgeDistBackward : public Node {
+  SavedVariable x;
+  c10::intrusive_ptr<EdgeGraph> graph;
+
+  std::string name() const override { return "EdgeDistancesBackward"; }
+  void release_variables() override { x.reset_data(); }
+  variable_list apply(variable_list&& grads) override {
+    if (!grads[0].defined()) return variable_list(1);
+    const Tensor v = x.unpack();
     const EdgeGraph& e = *graph;
-    const int64_t dim = x.size(1);
-    const c10::cuda::CUDAGuard guard(x.device());
-    Tensor dx = e.m ? at::empty({e.n, dim}, x.options()) : at::zeros({e.n, dim}, x.options());
+    const int64_t dim = v.size(1);
+    const c10::cuda::CUDAGuard guard(v.device());
+    Tensor dx = e.m ? at::empty({e.n, dim}, v.options()) : at::zeros({e.n, dim}, v.options());
     if (e.m) {
       e.use();
-      const Rows t = as_rows(x, dim);
+      const Rows t = as_rows(v, dim);
       const Tensor g = grads[0].contiguous();
-      const int code = code_of(x.scalar_type());
+      const int code = code_of(v.scalar_type());
       const size_t nb = lg_edge_sqdist_grad_workspace_bytes((int)e.nchunks, (int)dim, code);
-      const Tensor ws = nb ? bytes(nb, x) : Tensor();
+      const Tensor ws = nb ? bytes(nb, v) : Tensor();
       auto list = [](const Tensor& l) { return l.defined() ? l.data_ptr<int>() : nullptr; };
       check_status(lg_edge_sqdist_grad(e.n, e.m, (int)dim, code, e.rowptr.data_ptr<int>(), e.other(), e.eid(),
                                        (int)e.nlong, list(e.long_row), list(e.long_first), (int)e.nchunks,
                                        list(e.chunk_row), list(e.chunk_first), t.t.data_ptr(), t.ld, g.data_ptr(),
-                                       dx.data_ptr(), ptr(ws), nb, stream_of(x)));
+                                       dx.data_ptr(), ptr(ws), nb, stream_of(v)));
     }
-    return once({dx, Tensor()});
+    return once({dx});
   }
 };
 
@@ -428,8 +449,19 @@ Tensor edge_sqdist(const Tensor& x, const c10::intrusive_ptr<EdgeGraph>& g) {
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == g->n && x.size(1) >= 1 && x.size(1) <= (1 << 20), "x must be (", g->n,
                     ", dim), got shape ", x.sizes());
   TORCH_CHECK_VALUE(x.device() == g->device, "x is on ", x.device(), ", the edges on ", g->device);
-  if (at::GradMode::is_enabled() && x.requires_grad()) return EdgeDist::apply(x, g);
-  return edge_forward(x, *g);
+  const bool differentiate = at::GradMode::is_enabled() && wants_grad(x);
+  Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    out = edge_forward(x, *g);
+  }
+  if (differentiate) {
+    auto node = node_of<EdgeDistBackward>(x);
+    node->x = SavedVariable(x, false);
+    node->graph = g;
+    torch::autograd::set_history(out, node);
+  }
+  return out;
 }
 
 }  // namespace
