@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
 }
 
 // ---------------------------------------------------------------------------
-// The same sort in one launch, by one cluster: up to kClusterMost ids in 8
-// blocks, up to kBlockMost in one.  The blocks exchange their digit counts
+// The same sort in one launch, by one cluster of 1, 4 or 8 blocks, for up to
+// kClusterMost ids.  The blocks exchange their digit counts
 // through distributed shared memory and the pairs through L2; a cluster barrier
 // stands where the other form has a launch.  Digits of up to 10 bits, so two
 // passes for up to 2^20 rows.  Every thread keeps its ITEMS pairs and their places
@@ -315,7 +315,6 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterCtas = 8;
-constexpr int kBlockMost = 4 * kClusterThreads;
 constexpr int kClusterMost = 16 * kClusterThreads * kClusterCtas;
 
 struct ClusterSortArgs {
@@ -451,7 +450,10 @@ __global__ void __launch_bounds__(kSmallMost) sort_small_kernel(ClusterSortArgs 
   c.buf[0][place] = kv;
 }
 
-constexpr int kFillCtas = 128;
+// Blocks of a sort with clearing.  Clusters of 4 find room on nearly all SMs, which
+// clears 128 MB beside the sort of 16384 ids in 26 us; clusters of 8 took 41 us, and
+// the sort alone takes 23 us with either.
+constexpr int kFillCtas = 144;
 
 template <int ITEMS> cudaError_t launch_cluster_sort(const ClusterSortArgs& c, int ctas, cudaStream_t st) {
   const int smem = (int)sizeof(unsigned) * ((kClusterWarps + kClusterCtas) << c.width);
@@ -460,8 +462,7 @@ template <int ITEMS> cudaError_t launch_cluster_sort(const ClusterSortArgs& c, i
                                  (int)sizeof(unsigned) * ((kClusterWarps + kClusterCtas) << 10));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  // clusters of 8 find room on 16 x 8 SMs; the first one sorts
-  cfg.gridDim = dim3(c.fill.bytes ? kFillCtas : ctas);
+  cfg.gridDim = dim3(c.fill.bytes ? kFillCtas : ctas);   // the first cluster sorts
   cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -523,9 +524,11 @@ cudaError_t sort_ids(long long rows, long long n, const void* ids, int ids64, lo
       return cudaGetLastError();
     }
     *sorted = buf[(c.passes - 1) & 1];
-    if (n <= kBlockMost) return launch_cluster_sort<4>(c, 1, st);
-    if (n <= 4 * kClusterThreads * kClusterCtas) return launch_cluster_sort<4>(c, kClusterCtas, st);
-    return launch_cluster_sort<16>(c, kClusterCtas, st);
+    constexpr long long four = 4 * kClusterThreads;   // ids of a block
+    if (n <= four && !fill.bytes) return launch_cluster_sort<4>(c, 1, st);
+    if (n <= 4 * four) return launch_cluster_sort<4>(c, 4, st);
+    if (n <= 8 * four) return launch_cluster_sort<4>(c, 8, st);
+    return launch_cluster_sort<16>(c, 8, st);
   }
   if (nzero) {
     const cudaError_t e = cudaMemsetAsync(zero, 0, sizeof(unsigned) * (size_t)nzero, st);
@@ -877,7 +880,7 @@ constexpr int kSms = 148;   // of a B200
 // Bytes cleared beside the sort: about what the SMs that do not sort write in its
 // time.  131072 x 2048 bf16 with 16384 ids: 146 us with none, 130 us with all 537 MB
 // cleared there.
-constexpr long long kSideFillMost = 96LL << 20;
+constexpr long long kSideFillMost = 128LL << 20;
 
 SumPlan sum_plan(long long n, int nv, long long row_bytes) {
   SumPlan p;
