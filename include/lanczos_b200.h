@@ -522,7 +522,7 @@ int lg_rows_scatter(long long rows, int dim, int dtype, const void* table, long 
 int lg_layer_norm_forward(long long rows, int dim, int dtype, const void* x, long long ld_x, int param_dtype,
                           const void* weight, const void* bias, double eps, void* y, void* mean, void* rstd,
                           void* stream);
-size_t lg_layer_norm_workspace_bytes(long long rows, int dim, int dtype);   /* only for d_weight or d_bias */
+size_t lg_layer_norm_workspace_bytes(long long rows, int dim, int dtype);
 int lg_layer_norm_backward(long long rows, int dim, int dtype, const void* x, long long ld_x, const void* g,
                            long long ld_g, int param_dtype, const void* weight, const void* mean, const void* rstd,
                            void* dx, void* d_weight, void* d_bias, void* ws, size_t ws_bytes, void* stream);

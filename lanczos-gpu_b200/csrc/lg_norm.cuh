@@ -18,8 +18,7 @@
 // Teams: part of a warp for short rows (the fewest lanes that hold the row with
 // at most four vectors each: the more rows a warp holds, the fewer times it
 // issues the divide and square root of a row), a block for long ones.  Rows too
-// long for a block's registers go through the *_long kernels, which read the
-// row again for every pass (from L2).
+// long for a block's registers are read again for every pass (from L2).
 #pragma once
 
 #include "lg_feat.cuh"
@@ -343,6 +342,11 @@ int norm_parts(long long rows, int dim, int sms) {
   per_sm = per_sm < 4 ? 4 : per_sm > 32 ? 32 : per_sm;
   const long long most = (long long)sms * per_sm;
   return (int)(rows < most ? rows : most);
+}
+
+// The means of long rows (two a row), then the partial rows.
+size_t norm_workspace(long long rows, int dim, int dtype, int sms) {
+  return align_up((size_t)rows * 2 * acc_size(dtype)) + (size_t)norm_parts(rows, dim, sms) * 2 * dim * acc_size(dtype);
 }
 
 // F<T, P, V, K, BLOCK, AFFINE>(...) for the plan's K; K <= KM, part-warp teams at

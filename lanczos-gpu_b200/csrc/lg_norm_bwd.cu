@@ -131,56 +131,88 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_backward_kernel(
   }
 }
 
+// Rows too long for a block's registers, in two passes over x and g (the second
+// finds them in L2 where they fit): the two means of every row, a block of 1024
+// threads a row; then dx, dw and db by blocks that own 256 vectors of columns and
+// every gridDim.x-th row.
 template <typename T, typename P, int V>
-__global__ void __launch_bounds__(1024) norm_backward_long_kernel(NormArgs a, const T* __restrict__ x,
-                                                                  const T* __restrict__ g,
-                                                                  const Acc<T>* __restrict__ mean,
-                                                                  const Acc<T>* __restrict__ rstd,
-                                                                  T* __restrict__ dx, Acc<T>* __restrict__ part) {
+__global__ void __launch_bounds__(1024) norm_means_kernel(NormArgs a, const T* __restrict__ x, const T* __restrict__ g,
+                                                          const Acc<T>* __restrict__ mean,
+                                                          const Acc<T>* __restrict__ rstd, Acc<T>* __restrict__ means) {
   typedef Acc<T> A;
+  typedef Lane<T, V> L;
   __shared__ __align__(16) A scratch[128];
   clear_scratch(scratch, 128);
   int half = 0;
   const A inv = (A)1 / (A)a.dim;
-  A* dw = part + (long long)blockIdx.x * 2 * a.dim;   // this block's sums, each column by one thread
-  A* db = dw + a.dim;
-  bool first = true;
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, first = false) {
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* px = x + row * a.ld_x;
     const T* pg = g + row * a.ld_g;
-    const A mu = mean[row], r = rstd[row];
-    A s[2] = {0, 0};
+    const L minus = spread<L>(-mean[row]), rr = spread<L>(rstd[row]);
+    L s0 = spread<L>((A)0), s1 = s0;
     for (int c = threadIdx.x; c < a.nv; c += 1024) {
       const Vec<T, V> vx = load_vec<T, V>(px + (long long)c * V), vg = load_vec<T, V>(pg + (long long)c * V);
       Params<P, V> w;
-      if (a.w) w.load(static_cast<const P*>(a.w) + (long long)c * V);
+      w.load_or(a.w, (long long)c * V, 1.0f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const A h = (to_acc(vx.v[i]) - mu) * r, gv = to_acc(vg.v[i]);
-        const A wg = a.w ? gv * to_acc(w.value(i)) : gv;
-        s[0] += wg;
-        s[1] += wg * h;
-        const long long o = (long long)c * V + i;
-        if (a.want_dw) dw[o] = (first ? (A)0 : dw[o]) + gv * h;
-        if (a.want_db) db[o] = (first ? (A)0 : db[o]) + gv;
+      for (int n = 0; n < lanes<V>; ++n) {
+        const L wg = mul(widen<T, V>(vg.v, n), w.lane(n));
+        s0 = add(s0, wg);
+        s1 = fma(wg, mul(add(widen<T, V>(vx.v, n), minus), rr), s1);
       }
     }
-    if (!dx) continue;
+    A s[2] = {sum(s0), sum(s1)};
     team_sum<A, 2, true>(s, 0, scratch, half);
-    const A m0 = s[0] * inv, m1 = s[1] * inv;
-    for (int c = threadIdx.x; c < a.nv; c += 1024) {
-      const Vec<T, V> vx = load_vec<T, V>(px + (long long)c * V), vg = load_vec<T, V>(pg + (long long)c * V);
-      Params<P, V> w;
-      if (a.w) w.load(static_cast<const P*>(a.w) + (long long)c * V);
-      Vec<T, V> o;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const A h = (to_acc(vx.v[i]) - mu) * r, gv = to_acc(vg.v[i]);
-        const A wg = a.w ? gv * to_acc(w.value(i)) : gv;
-        o.v[i] = from_acc<T>(r * (wg - m0 - h * m1));
-      }
-      store_vec<T, V>(dx + row * a.dim + (long long)c * V, o);
+    if (threadIdx.x == 0) {
+      means[2 * row] = s[0] * inv;
+      means[2 * row + 1] = s[1] * inv;
     }
+  }
+}
+
+template <typename T, typename P, int V>
+__global__ void __launch_bounds__(256) norm_columns_kernel(NormArgs a, const T* __restrict__ x, const T* __restrict__ g,
+                                                           const Acc<T>* __restrict__ mean,
+                                                           const Acc<T>* __restrict__ rstd, const Acc<T>* __restrict__ means,
+                                                           T* __restrict__ dx, Acc<T>* __restrict__ part) {
+  typedef Acc<T> A;
+  typedef Lane<T, V> L;
+  constexpr int N = lanes<V>;
+  const int c = blockIdx.y * 256 + threadIdx.x;
+  if (c >= a.nv) return;
+  const long long col = (long long)c * V;
+  Params<P, V> w;
+  w.load_or(a.w, col, 1.0f);
+  L dw[N], db[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) dw[n] = db[n] = spread<L>((A)0);
+#pragma unroll 4
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const Vec<T, V> vx = load_vec<T, V>(x + row * a.ld_x + col), vg = load_vec<T, V>(g + row * a.ld_g + col);
+    const L minus = spread<L>(-mean[row]), rr = spread<L>(rstd[row]);
+    L m0 = spread<L>((A)0), m1 = m0;
+    if (dx) {
+      m0 = spread<L>(-means[2 * row]);
+      m1 = spread<L>(-means[2 * row + 1]);
+    }
+    Vec<T, V> o;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const L h = mul(add(widen<T, V>(vx.v, n), minus), rr), gv = widen<T, V>(vg.v, n);
+      dw[n] = fma(gv, h, dw[n]);
+      db[n] = add(db[n], gv);
+      narrow<T, V>(mul(rr, fma(h, m1, add(mul(gv, w.lane(n)), m0))), o.v, n);
+    }
+    if (dx) store_vec<T, V>(dx + row * a.dim + col, o);
+  }
+  A* out = part + (long long)blockIdx.x * 2 * a.dim;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (!(which ? a.want_db : a.want_dw)) continue;
+    Vec<A, V> o;
+#pragma unroll
+    for (int n = 0; n < N; ++n) narrow<A, V>(which ? db[n] : dw[n], o.v, n);
+    store_values<A, V>(out + (long long)which * a.dim + col, o);
   }
 }
 
@@ -201,13 +233,15 @@ cudaError_t launch_backward(const NormArgs& a, const NormPlan& p, const T* x, co
 
 template <typename T, typename P, int V>
 cudaError_t norm_backward_rows(NormArgs a, const T* x, const T* g, const Acc<T>* m, const Acc<T>* r, T* dx,
-                               Acc<T>* part, int* parts, int sms, cudaStream_t st) {
+                               Acc<T>* part, Acc<T>* means, int* parts, int sms, cudaStream_t st) {
   a.nv = a.dim / V;
   const NormPlan p = norm_plan(a.nv, KMax<T, V>::backward);
   a.lg = p.lg;
   if (p.k == 0) {
-    *parts = norm_grid(a.rows, p, sms, 1);
-    norm_backward_long_kernel<T, P, V><<<*parts, 1024, 0, st>>>(a, x, g, m, r, dx, part);
+    if (dx) norm_means_kernel<T, P, V><<<norm_grid(a.rows, p, sms, 2), 1024, 0, st>>>(a, x, g, m, r, means);
+    const int cols = (a.nv + 255) / 256, want = 4 * sms / cols > 1 ? 4 * sms / cols : 1;   // four blocks a SM
+    *parts = (int)(a.rows < want ? a.rows : want);
+    norm_columns_kernel<T, P, V><<<dim3(*parts, cols), 256, 0, st>>>(a, x, g, m, r, means, dx, part);
     return cudaGetLastError();
   }
   if constexpr (std::is_same<P, T>::value) {
@@ -222,10 +256,11 @@ template <typename T, typename P, int V>
 cudaError_t norm_backward(const NormArgs& a, const T* x, const T* g, const void* mean, const void* rstd, T* dx, void* dw,
                           void* db, void* ws, int sms, cudaStream_t st) {
   typedef Acc<T> A;
-  A* part = static_cast<A*>(ws);
+  A* means = static_cast<A*>(ws);   // two values a row, of long rows only
+  A* part = reinterpret_cast<A*>(static_cast<char*>(ws) + align_up((size_t)a.rows * 2 * sizeof(A)));
   int parts = 0;
   const cudaError_t e = norm_backward_rows<T, P, V>(a, x, g, static_cast<const A*>(mean), static_cast<const A*>(rstd),
-                                                    dx, part, &parts, sms, st);
+                                                    dx, part, means, &parts, sms, st);
   if (e != cudaSuccess || (!dw && !db)) return e;
   // dw and db lie side by side in a partial row: one sum over both, or over one of them
   const int dim = a.dim;
@@ -244,7 +279,7 @@ extern "C" size_t lg_layer_norm_workspace_bytes(long long rows, int dim, int dty
   if (!norm_args_ok(rows, dim, dtype, dtype)) return 0;
   const int sms = sm_count();
   if (sms < 1) return 0;
-  return (size_t)norm_parts(rows, dim, sms) * 2 * dim * acc_size(dtype);
+  return norm_workspace(rows, dim, dtype, sms);
 }
 
 extern "C" int lg_layer_norm_backward(long long rows, int dim, int dtype, const void* x, long long ld_x, const void* g,
@@ -252,11 +287,11 @@ extern "C" int lg_layer_norm_backward(long long rows, int dim, int dtype, const 
                                       const void* rstd, void* dx, void* d_weight, void* d_bias, void* ws,
                                       size_t ws_bytes, void* stream) {
   if (!norm_args_ok(rows, dim, dtype, param_dtype) || !x || !g || ld_x < dim || ld_g < dim || !mean || !rstd ||
-      (!dx && !d_weight && !d_bias) || ((d_weight || d_bias) && !ws))
+      (!dx && !d_weight && !d_bias) || !ws)
     return bad_args("lg_layer_norm_backward: invalid arguments");
   const int sms = sm_count();
   if (sms < 1) return bad_args("lg_layer_norm_backward: no CUDA device");
-  if ((d_weight || d_bias) && ws_bytes < (size_t)norm_parts(rows, dim, sms) * 2 * dim * acc_size(dtype))
+  if (ws_bytes < norm_workspace(rows, dim, dtype, sms))
     return bad_args("lg_layer_norm_backward: workspace too small");
   NormArgs a = {};
   a.rows = rows;

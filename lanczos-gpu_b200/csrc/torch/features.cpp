@@ -276,12 +276,8 @@ struct LayerNormBackward : public Node {
     if (rows && (dx.defined() || dw.defined() || db.defined())) {
       const Rows t = as_rows(v, dim), g = as_rows(grads[0], dim);
       const int code = code_of(v.scalar_type());
-      size_t nb = 0;
-      Tensor ws;
-      if (dw.defined() || db.defined()) {
-        nb = lg_layer_norm_workspace_bytes(rows, (int)dim, code);
-        ws = bytes(nb, v);
-      }
+      const size_t nb = lg_layer_norm_workspace_bytes(rows, (int)dim, code);
+      const Tensor ws = bytes(nb, v);
       const char* mean = static_cast<const char*>(s.data_ptr());
       check_status(lg_layer_norm_backward(rows, (int)dim, code, t.t.data_ptr(), t.ld, g.t.data_ptr(), g.ld, code_of(params),
                                           ptr(w), mean, mean + rows * s.element_size(), ptr(dx), ptr(dw), ptr(db), ptr(ws),
