@@ -145,17 +145,16 @@ template <bool BLOCK> struct Team {
 };
 
 // The rows that a block takes next, on their way to shared memory while one is
-// worked on: `stages` rows of K vectors of each of NA arrays.  Every thread
+// worked on: two rows of K vectors of each of NA arrays.  Every thread
 // copies the vectors that it will read itself, so its own wait is all the
 // ordering it needs.  What is in flight is then not limited by the registers
-// (16384 x 4096 bf16 forward: 93 us with loads to registers, 53 us with four
-// stages).  Narrower accesses and part-warp teams load to registers when they
-// need a row: a 4-byte asynchronous copy moves a quarter of a line's sectors at a
-// time (5003 x 1537 fp32 forward: 28 us with them, 19.5 us with loads), and short
-// rows have enough warps.
+// (16384 x 4096 bf16 forward: 93 us with loads to registers, 42 us so).  Narrower
+// accesses and part-warp teams load to registers when they need a row: a 4-byte
+// asynchronous copy moves a quarter of a line's sectors at a time (5003 x 1537 fp32
+// forward: 28 us with them, 17 us with loads), and short rows have enough warps.
 template <typename T, int V, int K, int NA, bool BLOCK> struct Rows {
   static constexpr bool async = BLOCK && sizeof(T) * V == 16;
-  static constexpr int stages = 16 * NA * K >= 128 ? 2 : 4;   // 512 threads take at most 128 KB
+  static constexpr int stages = 2;
   typedef Acc<T> A;
   static constexpr int stats = NA - 1;   // with g (NA = 2) a row's mean and 1 / deviation come along
   const T* src[NA];        // this thread's first vector of the next row to fetch
@@ -278,13 +277,15 @@ struct NormPlan {
   int block, lg, k, threads, per;   // k = 0: the long kernels; per: rows of a block at a time
 };
 
-// Part-warp teams: the fewest lanes with at most four vectors each, so that a
-// warp's loads stay whole lines.  Blocks: 128 threads if they hold the row, since a
-// row's two sums over the block cost a thread as much as eight elements do.
+// Rows of at most a warp of vectors go to part-warp teams: the fewest lanes with at
+// most four vectors each, so that a warp's loads stay whole lines.  Longer ones go to
+// blocks, of as few threads as hold them with four vectors each (two where the
+// backward pass keeps so many), since a row's two sums over the block cost a thread
+// as much as eight elements do.
 NormPlan norm_plan(int nv, int kmax) {
   NormPlan p;
   const int kw = kmax < 4 ? kmax : 4;
-  p.block = nv > 32 * kw;
+  p.block = nv > 32;
   p.lg = 0;
   p.threads = 256;
   int k;
@@ -293,7 +294,8 @@ NormPlan norm_plan(int nv, int kmax) {
     k = (nv + (1 << p.lg) - 1) >> p.lg;
   } else {
     k = 1;
-    while (k < kmax && nv > 128 * k) k *= 2;
+    while (k < kw && nv > 32 * k) k *= 2;
+    while (k < kmax && nv > 256 * k) k *= 2;
     p.threads = ((nv + k - 1) / k + 31) / 32 * 32;
     if (p.threads > kBlock) k = 0;
   }
@@ -326,6 +328,16 @@ struct Resident {
     return b;
   }
 };
+
+// Blocks a SM that keep 32 KB of rows on their way (vectors of 16 bytes a thread):
+// more of them read no faster but worse.  16384 x 2048 fp32 forward: 43 us with 32
+// KB, 48 us with 56 KB; 16384 x 4096 bf16: 42 us with 32 KB, 51 us with 96 KB (four
+// rows a block instead of two).
+int in_flight(int per_sm, int threads, int vectors) {
+  const int most = 2048 / (threads * vectors);
+  const int cap = most > 2 ? most : 2;   // two, so that one block's sums run beside the other's loads
+  return per_sm < cap ? per_sm : cap;
+}
 
 // Every block of a persistent grid is resident: `per_sm` of them on an SM.
 int norm_grid(long long rows, const NormPlan& p, int sms, int per_sm) {

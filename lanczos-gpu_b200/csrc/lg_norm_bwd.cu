@@ -226,6 +226,7 @@ cudaError_t launch_backward(const NormArgs& a, const NormPlan& p, const T* x, co
   int per_sm = res.get(reinterpret_cast<const void*>(f), p.threads, smem);
   if (per_sm < 1) return cudaErrorInvalidConfiguration;
   if (per_sm > 1024 / p.threads) per_sm = 1024 / p.threads;
+  if (Rows<T, V, K, 2, BLOCK>::async) per_sm = in_flight(per_sm, p.threads, 2 * K);
   *parts = norm_grid(a.rows, p, sms, per_sm);
   f<<<*parts, p.threads, smem, st>>>(a, x, g, mean, rstd, dx, part);
   return cudaGetLastError();

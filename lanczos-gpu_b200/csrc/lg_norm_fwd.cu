@@ -153,8 +153,9 @@ cudaError_t launch_forward(const NormArgs& a, const NormPlan& p, const T* x, T* 
   static Resident res;
   void (*f)(NormArgs, const T*, T*, Acc<T>*, Acc<T>*) = norm_forward_kernel<T, P, V, K, BLOCK, AFFINE>;
   const size_t smem = Rows<T, V, K, 1, BLOCK>::bytes(p.threads);
-  const int per_sm = res.get(reinterpret_cast<const void*>(f), p.threads, smem);
+  int per_sm = res.get(reinterpret_cast<const void*>(f), p.threads, smem);
   if (per_sm < 1) return cudaErrorInvalidConfiguration;
+  if (Rows<T, V, K, 1, BLOCK>::async) per_sm = in_flight(per_sm, p.threads, K);
   const int grid = norm_grid(a.rows, p, sms, per_sm);
   f<<<grid, p.threads, smem, st>>>(a, x, y, mean, rstd);
   return cudaGetLastError();
