@@ -149,8 +149,10 @@ Tensor gather(const Tensor& table, const Tensor& column, const Tensor& ids, cons
 }
 
 struct LookupBackward : public Node {
-  SavedVariable table, column, ids;
+  SavedVariable table, column, ids;   // the table only for the scale's gradient
   LookupArgs args;
+  int64_t rows = 0, dim = 0;
+  at::TensorOptions options;
 
   std::string name() const override { return "EmbeddingLookupBackward"; }
   void release_variables() override {
@@ -161,20 +163,22 @@ struct LookupBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(2);
     if (!grads[0].defined()) return out;
-    const Tensor w = table.unpack(), c = column.unpack(), at = ids.unpack();
-    const int64_t rows = w.size(0), dim = w.size(1), n = at.numel();
-    const int code = code_of(w.scalar_type());
+    const Tensor c = column.unpack(), at = ids.unpack();
+    const int64_t n = at.numel();
+    const int code = code_of(options.dtype().toScalarType());
     const bool want_table = task_should_compute_output(0), want_scale = c.defined() && task_should_compute_output(1);
-    const c10::cuda::CUDAGuard guard(w.device());
-    if (want_table) out[0] = n ? at::empty({rows, dim}, w.options()) : at::zeros({rows, dim}, w.options());
+    const c10::cuda::CUDAGuard guard(options.device());
+    if (want_table) out[0] = n ? at::empty({rows, dim}, options) : at::zeros({rows, dim}, options);
     if (want_scale) out[1] = n ? at::empty({dim}, c.options()) : at::zeros({dim}, c.options());
     if (n && (want_table || want_scale)) {
-      const Rows g = as_rows(grads[0], dim), t = as_rows(w, dim);
+      const Rows g = as_rows(grads[0], dim);
+      Rows t = {Tensor(), dim};
+      if (want_scale) t = as_rows(table.unpack(), dim);
       const size_t nb = lg_rows_scatter_workspace_bytes(rows, (int)dim, code, n, want_scale);
-      const Tensor ws = bytes(nb, w);
-      check_status(lg_rows_scatter(rows, (int)dim, code, t.t.data_ptr(), t.ld, n, at.data_ptr(),
-                                   at.scalar_type() == at::kLong, args.mode, ptr(c), args.value, args.has_pad, args.pad,
-                                   g.t.data_ptr(), g.ld, ptr(out[0]), ptr(out[1]), ws.data_ptr(), nb, stream_of(w)));
+      const Tensor ws = bytes(nb, at);
+      check_status(lg_rows_scatter(rows, (int)dim, code, ptr(t.t), t.ld, n, at.data_ptr(), at.scalar_type() == at::kLong,
+                                   args.mode, ptr(c), args.value, args.has_pad, args.pad, g.t.data_ptr(), g.ld, ptr(out[0]),
+                                   ptr(out[1]), ws.data_ptr(), nb, stream_of(at)));
     }
     return once(std::move(out));
   }
@@ -216,7 +220,10 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, const std::optio
   }
   if (differentiate) {
     auto node = node_of<LookupBackward>(table, column);
-    node->table = SavedVariable(table, false);
+    if (wants_grad(column)) node->table = SavedVariable(table, false);
+    node->rows = table.size(0);
+    node->dim = dim;
+    node->options = table.options();
     node->column = SavedVariable(column, false);
     node->ids = SavedVariable(at, false);
     node->args = a;

@@ -49,7 +49,9 @@ def _scalar(t) -> float:
 
 def _rows(X: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
     """X[at] for an (n, B) block: the library's row lookup."""
-    return embedding_lookup(X, at) if X.dim() == 2 and X.numel() else X.index_select(0, at)
+    if X.dim() == 2 and X.numel() and X.dtype in (torch.float32, torch.float64):
+        return embedding_lookup(X, at)
+    return X.index_select(0, at)
 
 
 class ImgpPrecisionMatvec:

@@ -151,6 +151,34 @@ def test_lookup_runs_at_tile_borders(n):
         lookup_case(torch.float32, rows, 6, n, kind, "column", seed=n)
 
 
+@pytest.mark.parametrize("n,kind", [(3, "uniform"), (700, "zipf"), (5000, "zipf"), (20000, "uniform"), (40000, "zipf"),
+                                    (140000, "zipf")])
+def test_lookup_large_tables(n, kind):
+    """Tables beyond what is cleared beside the sort, of odd rows too; every way of sorting."""
+    lookup_case(torch.bfloat16, 70001, 1024 if n < 100000 else 8, n, kind, "number", pad=70000, seed=n)
+    lookup_case(torch.float32, 60011, 601 if n < 10000 else 33, n, kind, "none", seed=n + 1)
+
+
+def test_lookup_saves_only_what_its_gradient_needs():
+    """The table may change between the passes unless the scale's gradient reads it."""
+    from gpu_eigsh.features import embedding_lookup
+
+    ids = make_ids("zipf", 20, 50, 1)
+    W = randn((20, 6), torch.float32, 2).requires_grad_(True)
+    s = randn((6,), torch.float32, 3).requires_grad_(True)
+    g = randn((50, 6), torch.float32, 4)
+    ref = torch.autograd.grad(embedding_lookup(W, ids, s.detach()), [W], g)[0]
+    y = embedding_lookup(W, ids, s.detach())
+    with torch.no_grad():
+        W.add_(1.0)
+    assert torch.equal(torch.autograd.grad(y, [W], g)[0], ref)
+    y = embedding_lookup(W, ids, s)
+    with torch.no_grad():
+        W.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, [W, s], g)
+
+
 def test_lookup_all_tokens_are_padding():
     from gpu_eigsh.features import embedding_lookup
 
