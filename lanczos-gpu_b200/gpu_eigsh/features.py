@@ -20,7 +20,8 @@ are in float32 (float64 for float64), each result is rounded once.  Sums run
 in a fixed order, so equal inputs give equal bits.  Calls run on the current
 stream of their tensors' device, allocate from torch and wait for nothing
 (``EdgeDistances`` checks its indices when it is built, which waits once; the
-rest can be captured into CUDA graphs).  The gradients are not differentiable
+rest can be captured into CUDA graphs; as with torch's own operations, capture a
+backward pass only when no eager autograd graph of the same leaves is alive).  The gradients are not differentiable
 themselves (a second backward pass raises).  There is no CPU implementation.
 
 Squared distances are the ``x_edge_dists`` of
