@@ -538,15 +538,18 @@ size_t lg_edge_graph_workspace_bytes(long long n, long long m);
 int lg_edge_graph(long long n, long long m, const long long* idx, int* ends, int* rowptr, int* other, int* eid,
                   int* bad, void* ws, size_t ws_bytes, void* stream);
 /* d2[e] = |x[begin_e, :] - x[end_e, :]|^2 in the accumulation type: the
- * x_edge_dists of the IMGP operator.  Rows of x lie less than 4 GiB apart. */
+ * x_edge_dists of the IMGP operator.  Rows of x lie less than 4 GiB apart.  The
+ * workspace (0 bytes for most x) takes a copy of rows that are not aligned. */
+size_t lg_edge_sqdist_workspace_bytes(long long n, long long m, int dim, int dtype, const void* x, long long ld_x);
 int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x, long long ld_x,
-                   void* d2, void* stream);
+                   void* d2, void* ws, size_t ws_bytes, void* stream);
 /* dx[v, :] = 2 sum over the edges e at v of g[e] (x[v, :] - x[other end, :]),
  * g = dL/d d2.  The vertices with more than LG_EDGE_CHUNK edges are listed by
  * the caller: long_row (nlong vertices), long_first (index of each one's first
  * chunk), and for each of the nchunks pieces of LG_EDGE_CHUNK list entries
  * (vertex by vertex) chunk_row and chunk_first (its first position in eid). */
-size_t lg_edge_sqdist_grad_workspace_bytes(int nchunks, int dim, int dtype);
+size_t lg_edge_sqdist_grad_workspace_bytes(long long n, long long m, int dim, int dtype, const void* x, long long ld_x,
+                                           int nchunks);
 int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype, const int* rowptr, const int* other,
                         const int* eid, int nlong, const int* long_row, const int* long_first, int nchunks,
                         const int* chunk_row, const int* chunk_first, const void* x, long long ld_x, const void* g,

@@ -13,8 +13,12 @@
 // rest.
 //
 // Both directions are bound by the gathers of x rows from L2: by their latency, so
-// a group keeps several edges' rows in flight, and by the instructions around
-// them, so a lane takes two vectors of a row where the row has them.
+// a group keeps several edges' rows in flight; by the sectors that they touch; and by
+// the instructions around them, so a lane takes two vectors of a row where the row
+// has more than two.  10^6 vertices, 5 10^6 edges with far ends, 10 fp32: forward
+// 84 us, backward 136 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
+// pieces take the same, and a lane a vector costs 240 us instead of 220.  10^5
+// vertices, 10^6 edges, 64 fp32: 95 us for both.
 #include "lg_feat.cuh"
 
 #include "../../include/lanczos_b200.h"
@@ -71,6 +75,21 @@ struct EdgeArgs {
   unsigned stride;       // bytes from one row of x to the next
   int nv, lg;
 };
+
+// The rows of x from 16-byte boundaries, filled up with zeros: a thread makes one
+// vector.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) edge_pack_kernel(long long n, int dim, int nv, const T* __restrict__ x,
+                                                             long long ld, T* __restrict__ out) {
+  for (long long t = (long long)blockIdx.x * kThreads + threadIdx.x; t < n * nv; t += (long long)gridDim.x * kThreads) {
+    const long long row = t / nv;
+    const int c = (int)(t - row * nv) * V;
+    Vec<T, V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = c + k < dim ? x[row * ld + c + k] : from_acc<T>((Acc<T>)0);
+    store_vec<T, V>(out + t * V, o);
+  }
+}
 
 template <typename T> __device__ __forceinline__ const T* row_at(const T* x, int i, unsigned stride) {
   return reinterpret_cast<const T*>(reinterpret_cast<const char*>(x) + (unsigned long long)(unsigned)i * stride);
@@ -134,6 +153,7 @@ __global__ void __launch_bounds__(kThreads) edge_dist_kernel(EdgeArgs a, const i
 // ---------------------------------------------------------------------------
 struct GradArgs {
   EdgeArgs e;
+  int dim;               // columns of dx; at most e.nv vectors
   int nchunks;
   const int *rowptr, *other, *eid, *chunk_row, *chunk_first;
 };
@@ -141,7 +161,8 @@ struct GradArgs {
 // First the chunks, then the vertices.  A vertex row is written to dx, a chunk's
 // sum to part.  The indices of a batch of list entries are fetched while the rows
 // of the batch before are worked on.
-template <typename T, int V, int K>
+// WHOLE: whole vectors of dx can be stored.
+template <typename T, int V, int K, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) edge_grad_kernel(GradArgs a, const T* __restrict__ x,
                                                              const Acc<T>* __restrict__ g, T* __restrict__ dx,
                                                              Acc<T>* __restrict__ part) {
@@ -210,28 +231,33 @@ __global__ void __launch_bounds__(kThreads) edge_grad_kernel(GradArgs a, const T
       }
     }
   }
-  const long long dim = (long long)a.e.nv * V;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (!on[k]) continue;
     if (chunk) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) narrow<A, V>(acc[k][n], part + unit * dim + at[k], n);
+      for (int n = 0; n < N; ++n) narrow<A, V>(acc[k][n], part + unit * a.e.nv * V + at[k], n);
     } else {
       Vec<T, V> o;
       const L two = spread<L>((A)2);
 #pragma unroll
       for (int n = 0; n < N; ++n) narrow<T, V>(mul(acc[k][n], two), o.v, n);
-      store_vec<T, V>(dx + v * dim + at[k], o);
+      if (WHOLE) {
+        store_vec<T, V>(dx + v * ((long long)a.e.nv * V) + at[k], o);
+      } else {
+#pragma unroll
+        for (int n = 0; n < V; ++n)
+          if (at[k] + n < a.dim) dx[v * a.dim + at[k] + n] = o.v[n];
+      }
     }
   }
 }
 
 // The long vertices: a block adds 32 columns of a vertex's chunks (from
-// long_first[r] on, one after the other), eight rows of threads taking every
-// eighth chunk.
+// long_first[r] on, one after the other, pitch columns each), eight rows of
+// threads taking every eighth chunk.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) edge_long_kernel(int dim, const int* __restrict__ rowptr,
+__global__ void __launch_bounds__(kThreads) edge_long_kernel(int dim, long long pitch, const int* __restrict__ rowptr,
                                                              const int* __restrict__ long_row,
                                                              const int* __restrict__ long_first, const Acc<T>* part,
                                                              T* __restrict__ dx) {
@@ -245,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) edge_long_kernel(int dim, const int*
     Acc<T> s = 0;
     if (c < dim) {
 #pragma unroll 4
-      for (int k = grp; k < count; k += kThreads / 32) s += part[(q0 + k) * dim + c];
+      for (int k = grp; k < count; k += kThreads / 32) s += part[(q0 + k) * pitch + c];
     }
     __syncthreads();
     red[grp][lane] = s;
@@ -268,7 +294,7 @@ int group_log(int nv) {
 
 template <typename T, int V>
 cudaError_t edge_dist(EdgeArgs a, int dim, const int* ends, const T* x, void* d2, cudaStream_t st) {
-  a.nv = dim / V;
+  a.nv = (dim + V - 1) / V;
   a.lg = group_log(a.nv);
   const int per = (kThreads >> a.lg) * kEdges;
   const unsigned grid = (unsigned)((a.m + per - 1) / per);
@@ -288,20 +314,23 @@ template <typename T, int V>
 cudaError_t edge_grad(GradArgs a, int dim, const T* x, const void* g, T* dx, const LongLists& l, void* ws,
                       cudaStream_t st) {
   typedef Acc<T> A;
-  a.e.nv = dim / V;
-  a.e.lg = group_log(a.e.nv);
+  a.e.nv = (dim + V - 1) / V;
+  a.e.lg = a.e.nv == 2 ? 1 : group_log(a.e.nv);
   const int ngrp = kThreads >> a.e.lg;
   const unsigned cols = (unsigned)((a.e.nv + (2 << a.e.lg) - 1) / (2 << a.e.lg));
   A* part = static_cast<A*>(ws);
   const dim3 grid((unsigned)((a.e.n + a.nchunks + ngrp - 1) / ngrp), cols);
   const A* gv = static_cast<const A*>(g);
-  if (a.e.nv > 1) edge_grad_kernel<T, V, 2><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
-  else edge_grad_kernel<T, V, 1><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  const bool whole = dim % V == 0 && reinterpret_cast<uintptr_t>(dx) % (V * sizeof(T)) == 0;
+  if (a.e.nv > 2 && whole) edge_grad_kernel<T, V, 2, true><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  else if (a.e.nv > 2) edge_grad_kernel<T, V, 2, false><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  else if (whole) edge_grad_kernel<T, V, 1, true><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
+  else edge_grad_kernel<T, V, 1, false><<<grid, kThreads, 0, st>>>(a, x, gv, dx, part);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && l.nlong > 0) {
     const unsigned pieces = (unsigned)((dim + 31) / 32);
     e = launch_pdl(edge_long_kernel<T>, dim3((unsigned)l.nlong, pieces < 65535u ? pieces : 65535u), dim3(kThreads), 0, st,
-                   dim, a.rowptr, l.row, l.first, part, dx);
+                   dim, (long long)a.e.nv * V, a.rowptr, l.row, l.first, part, dx);
   }
   return e;
 }
@@ -313,6 +342,44 @@ bool edge_sizes_ok(long long n, long long m) {
 bool edge_args_ok(long long n, long long m, int dim, int dtype, long long ld) {
   return edge_sizes_ok(n, m) && dim >= 1 && dim <= (1 << 20) && elem_size(dtype) && ld >= dim &&
          ld * elem_size(dtype) < (1LL << 32);
+}
+
+// An x whose rows can be read only in narrow pieces is copied to aligned rows
+// first, where its 2 m gathers then take at least a piece less for every 3 bytes
+// copied.  Measured forward + backward, us, without and with the copy: 10^5 vertices,
+// 10^6 edges, 333 fp16 909 and 571, 33 fp32 201 and 122; 500,000 vertices, 10^6 edges,
+// 33 fp32 331 and 293; at a piece for 4 bytes (10^6 vertices, 5 10^6 edges, 7 fp64) 282
+// both.  Under 16 MB of gathers the second launch costs more than it saves; above
+// 8 GB the copy would burden the device's memory.
+size_t packed_bytes(const EdgeArgs& a, int dim, int dtype, const void* x, long long ld) {
+  const long long es = elem_size(dtype), v16 = (dim * es + 15) / 16;
+  Align al((int)es);
+  al.address(x);
+  al.elements(ld);
+  al.elements(dim);
+  const bool pays = 6.0 * (double)a.m * (double)(dim / al.vec() - v16) >= (double)a.n * (double)(dim * es + 16 * v16) &&
+                    a.m * dim * es >= (16LL << 20) && a.n <= (8LL << 30) / (16 * v16);
+  return pays ? (size_t)(a.n * v16 * 16) : 0;
+}
+
+template <typename T>
+cudaError_t pack(EdgeArgs& a, int dim, const void* x, long long ld, void* out, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const int nv = (dim + V - 1) / V;
+  const long long blocks = (a.n * nv + kThreads - 1) / kThreads;
+  a.stride = (unsigned)nv * 16;
+  edge_pack_kernel<T, V><<<(unsigned)(blocks < (1 << 30) ? blocks : (1 << 30)), kThreads, 0, st>>>(
+      a.n, dim, nv, static_cast<const T*>(x), ld, static_cast<T*>(out));
+  return cudaGetLastError();
+}
+
+cudaError_t pack_any(EdgeArgs& a, int dim, int dtype, const void* x, long long ld, void* out, cudaStream_t st) {
+  switch (dtype) {
+    case LG_F64: return pack<double>(a, dim, x, ld, out, st);
+    case LG_F32: return pack<float>(a, dim, x, ld, out, st);
+    case LG_F16: return pack<__half>(a, dim, x, ld, out, st);
+    default: return pack<__nv_bfloat16>(a, dim, x, ld, out, st);
+  }
 }
 
 int wide_grid(long long n) {
@@ -359,20 +426,35 @@ extern "C" int lg_edge_graph(long long n, long long m, const long long* idx, int
   return cuda_status(cudaGetLastError(), "lg_edge_graph");
 }
 
+extern "C" size_t lg_edge_sqdist_workspace_bytes(long long n, long long m, int dim, int dtype, const void* x,
+                                                long long ld_x) {
+  if (!edge_args_ok(n, m, dim, dtype, ld_x)) return 0;
+  EdgeArgs a = {};
+  a.n = n;
+  a.m = m;
+  return packed_bytes(a, dim, dtype, x, ld_x);
+}
+
 extern "C" int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x,
-                              long long ld_x, void* d2, void* stream) {
-  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !ends || !x || !d2)
+                              long long ld_x, void* d2, void* ws, size_t ws_bytes, void* stream) {
+  const size_t nb = lg_edge_sqdist_workspace_bytes(n, m, dim, dtype, x, ld_x);
+  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !ends || !x || !d2 || (nb && (!ws || ws_bytes < nb)))
     return bad_args("lg_edge_sqdist: invalid arguments");
   EdgeArgs a = {};
   a.n = n;
   a.m = m;
   a.stride = (unsigned)(ld_x * elem_size(dtype));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   Align al(elem_size(dtype));
   al.address(x);
   al.elements(ld_x);
   al.elements(dim);
-  const int vec = al.vec();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int vec = nb ? 16 / elem_size(dtype) : al.vec();
+  if (nb) {
+    const cudaError_t e = pack_any(a, dim, dtype, x, ld_x, ws, st);
+    if (e != cudaSuccess) return cuda_status(e, "lg_edge_sqdist");
+    x = ws;
+  }
   auto run = [&]() -> cudaError_t {
 #define LG_F(T, V) edge_dist<T, V>(a, dim, ends, static_cast<const T*>(x), d2, st)
     LG_EDGE_DISPATCH(LG_F)
@@ -381,8 +463,17 @@ extern "C" int lg_edge_sqdist(long long n, long long m, int dim, int dtype, cons
   return cuda_status(run(), "lg_edge_sqdist");
 }
 
-extern "C" size_t lg_edge_sqdist_grad_workspace_bytes(int nchunks, int dim, int dtype) {
-  return (size_t)(nchunks > 0 ? nchunks : 0) * (dim > 0 ? dim : 0) * acc_size(dtype);
+namespace {
+size_t part_bytes(int nchunks, int dim, int dtype) {
+  const size_t es = elem_size(dtype), wide = (dim * es + 15) / 16 * 16 / es;   // columns of packed rows
+  return align_up((size_t)nchunks * wide * acc_size(dtype));
+}
+}  // namespace
+
+extern "C" size_t lg_edge_sqdist_grad_workspace_bytes(long long n, long long m, int dim, int dtype, const void* x,
+                                                     long long ld_x, int nchunks) {
+  if (!edge_args_ok(n, m, dim, dtype, ld_x) || nchunks < 0) return 0;
+  return part_bytes(nchunks, dim, dtype) + lg_edge_sqdist_workspace_bytes(n, m, dim, dtype, x, ld_x);
 }
 
 extern "C" int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype, const int* rowptr, const int* other,
@@ -390,28 +481,36 @@ extern "C" int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype,
                                    const int* chunk_row, const int* chunk_first, const void* x, long long ld_x,
                                    const void* g, void* dx, void* ws, size_t ws_bytes, void* stream) {
   if (!edge_args_ok(n, m, dim, dtype, ld_x) || !rowptr || !other || !eid || !x || !g || !dx || nlong < 0 ||
-      nchunks < nlong ||
-      (nlong > 0 && (!long_row || !long_first || !chunk_row || !chunk_first || !ws ||
-                     ws_bytes < lg_edge_sqdist_grad_workspace_bytes(nchunks, dim, dtype))))
+      nchunks < nlong || (nlong > 0 && (!long_row || !long_first || !chunk_row || !chunk_first)))
     return bad_args("lg_edge_sqdist_grad: invalid arguments");
+  if (nlong == 0) nchunks = 0;
+  const size_t nb = lg_edge_sqdist_grad_workspace_bytes(n, m, dim, dtype, x, ld_x, nchunks);
+  if (nb && (!ws || ws_bytes < nb)) return bad_args("lg_edge_sqdist_grad: the workspace is too small");
   GradArgs a = {};
   a.e.n = n;
   a.e.m = m;
   a.e.stride = (unsigned)(ld_x * elem_size(dtype));
-  a.nchunks = nlong > 0 ? nchunks : 0;
+  a.dim = dim;
+  a.nchunks = nchunks;
   a.rowptr = rowptr;
   a.other = other;
   a.eid = eid;
   a.chunk_row = chunk_row;
   a.chunk_first = chunk_first;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   Align al(elem_size(dtype));
   al.address(x);
-  al.address(dx);
   al.elements(ld_x);
   al.elements(dim);
-  const int vec = al.vec();
+  int vec = al.vec();
+  if (nb > part_bytes(nchunks, dim, dtype)) {
+    void* packed = static_cast<char*>(ws) + part_bytes(nchunks, dim, dtype);
+    const cudaError_t e = pack_any(a.e, dim, dtype, x, ld_x, packed, st);
+    if (e != cudaSuccess) return cuda_status(e, "lg_edge_sqdist_grad");
+    x = packed;
+    vec = 16 / elem_size(dtype);
+  }
   const LongLists l = {nlong, long_row, long_first};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&]() -> cudaError_t {
 #define LG_F(T, V) edge_grad<T, V>(a, dim, static_cast<const T*>(x), g, static_cast<T*>(dx), l, ws, st)
     LG_EDGE_DISPATCH(LG_F)

@@ -411,8 +411,11 @@ Tensor edge_forward(const Tensor& x, const EdgeGraph& g) {
   if (g.m) {
     g.use();
     const Rows t = as_rows(x, x.size(1));
-    check_status(lg_edge_sqdist(g.n, g.m, (int)x.size(1), code_of(x.scalar_type()), g.ends.data_ptr<int>(), t.t.data_ptr(),
-                                t.ld, out.data_ptr(), stream_of(x)));
+    const int dim = (int)x.size(1), code = code_of(x.scalar_type());
+    const size_t nb = lg_edge_sqdist_workspace_bytes(g.n, g.m, dim, code, t.t.data_ptr(), t.ld);
+    const Tensor ws = nb ? bytes(nb, x) : Tensor();
+    check_status(lg_edge_sqdist(g.n, g.m, dim, code, g.ends.data_ptr<int>(), t.t.data_ptr(), t.ld, out.data_ptr(),
+                                ptr(ws), nb, stream_of(x)));
   }
   return out;
 }
@@ -435,7 +438,8 @@ struct EdgeDistBackward : public Node {
       const Rows t = as_rows(v, dim);
       const Tensor g = grads[0].contiguous();
       const int code = code_of(v.scalar_type());
-      const size_t nb = lg_edge_sqdist_grad_workspace_bytes((int)e.nchunks, (int)dim, code);
+      const size_t nb = lg_edge_sqdist_grad_workspace_bytes(e.n, e.m, (int)dim, code, t.t.data_ptr(), t.ld,
+                                                             e.nlong ? (int)e.nchunks : 0);
       const Tensor ws = nb ? bytes(nb, v) : Tensor();
       auto list = [](const Tensor& l) { return l.defined() ? l.data_ptr<int>() : nullptr; };
       check_status(lg_edge_sqdist_grad(e.n, e.m, (int)dim, code, e.rowptr.data_ptr<int>(), e.other(), e.eid(),

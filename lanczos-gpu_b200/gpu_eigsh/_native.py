@@ -181,8 +181,9 @@ SIGNATURES = {
     "lg_layer_norm_backward": (_I, [_L, _I, _I, _V, _L, _V, _L, _I, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),
     "lg_edge_graph_workspace_bytes": (_SZ, [_L, _L]),
     "lg_edge_graph": (_I, [_L, _L, _V, _V, _V, _V, _V, _V, _V, _SZ, _V]),
-    "lg_edge_sqdist": (_I, [_L, _L, _I, _I, _V, _V, _L, _V, _V]),
-    "lg_edge_sqdist_grad_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "lg_edge_sqdist_workspace_bytes": (_SZ, [_L, _L, _I, _I, _V, _L]),
+    "lg_edge_sqdist": (_I, [_L, _L, _I, _I, _V, _V, _L, _V, _V, _SZ, _V]),
+    "lg_edge_sqdist_grad_workspace_bytes": (_SZ, [_L, _L, _I, _I, _V, _L, _I]),
     "lg_edge_sqdist_grad": (_I, [_L, _L, _I, _I, _V, _V, _V, _I, _V, _V, _I, _V, _V, _V, _L, _V, _V, _V, _SZ, _V]),
     "lg_eigsh_adjoint": (_I, [_I, C.c_longlong, _V, _V, _V, _I, _V, _V, _V, _V, _V, _I, C.c_double, _PI, _V]),
     "compute_adjoint_eigsh": (_I, [_I, _I, _PI, _PI, _PD, _I, _PD, _PD, _PD, _PD, _PD, _I, C.c_double]),

@@ -88,7 +88,16 @@ def test_edge_calls_refuse():
                                            (4, 4, 3, 6, P, P, 3, P), (4, 4, 3, 0, None, P, 3, P),
                                            (4, 4, 3, 0, P, None, 3, P), (4, 4, 3, 0, P, P, 2, P),
                                            (4, 4, 3, 0, P, P, 3, None)):
-        assert L.lg_edge_sqdist(n, m, dim, dt, ends, x, ld, d2, None) == BAD
+        assert L.lg_edge_sqdist(n, m, dim, dt, ends, x, ld, d2, None, 0, None) == BAD
+
+    # rows of 333 halves can be read by twos only: a copy in rows of 672 bytes, where it pays
+    need = L.lg_edge_sqdist_workspace_bytes(100000, 1000000, 333, 2, P, 333)
+    assert need == 100000 * 672
+    assert L.lg_edge_sqdist_grad_workspace_bytes(100000, 1000000, 333, 2, P, 333, 3) >= need + 3 * 333 * 4
+    assert L.lg_edge_sqdist(100000, 1000000, 333, 2, P, P, 333, P, P, need - 1, None) == BAD
+    assert L.lg_edge_sqdist(100000, 1000000, 333, 2, P, P, 333, P, None, need, None) == BAD
+    for m, dim, ld in ((1000000, 336, 336), (30000, 333, 333), (1000000, 16, 16)):
+        assert L.lg_edge_sqdist_workspace_bytes(100000, m, dim, 2, P, ld) == 0
 
     def grad(n=4, m=4, dim=3, dt=0, rp=P, nlong=0, lr=None, nch=0, x=P, ld=3, g=P, dx=P, ws=None, nb=0):
         return L.lg_edge_sqdist_grad(n, m, dim, dt, rp, P, P, nlong, lr, lr, nch, lr, lr, x, ld, g, dx, ws, nb, None)

@@ -461,6 +461,16 @@ def test_edges_hubs(dt):
     edge_case(DT[dt], 70, 40000, 80, hubs=True)
 
 
+@pytest.mark.parametrize("dt,n,m,dim,hubs", [("f16", 2000, 27000, 333, False), ("bf16", 700, 130000, 65, True),
+                                             ("f32", 9000, 70000, 65, False), ("f32", 300, 90000, 50, True),
+                                             ("f32", 400, 1450000, 3, False), ("f64", 5000, 70000, 33, True)])
+def test_edges_of_rows_that_are_copied(dt, n, m, dim, hubs):
+    """Rows at odd addresses and enough edges: the calls read an aligned copy."""
+    x = randn((n, 2 * dim), DT[dt], 5)
+    edge_case(DT[dt], n, m, dim, hubs=hubs)
+    edge_case(DT[dt], n, m, dim, hubs=hubs, x=x[:, 1:dim + 1])
+
+
 @pytest.mark.parametrize("m", [127, 128, 129, 255, 256, 257, 511, 512, 513, 1025])
 def test_edges_list_lengths_around_a_chunk(m):
     """A star: its centre has m edges."""
