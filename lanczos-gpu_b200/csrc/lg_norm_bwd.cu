@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_backward_kernel(
 // Rows too long for a block's registers, in two passes over x and g (the second
 // finds them in L2 where they fit): the two means of every row, a block of 1024
 // threads a row; then dx, dw and db by blocks that own 256 vectors of columns and
-// every gridDim.x-th row.
+// every gridDim.y-th row.
 template <typename T, typename P, int V>
 __global__ void __launch_bounds__(1024) norm_means_kernel(NormArgs a, const T* __restrict__ x, const T* __restrict__ g,
                                                           const Acc<T>* __restrict__ mean,
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(NormArgs a, const T* 
   typedef Acc<T> A;
   typedef Lane<T, V> L;
   constexpr int N = lanes<V>;
-  const int c = blockIdx.y * 256 + threadIdx.x;
+  const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.nv) return;
   const long long col = (long long)c * V;
   Params<P, V> w;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(NormArgs a, const T* 
 #pragma unroll
   for (int n = 0; n < N; ++n) dw[n] = db[n] = spread<L>((A)0);
 #pragma unroll 4
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const Vec<T, V> vx = load_vec<T, V>(x + row * a.ld_x + col), vg = load_vec<T, V>(g + row * a.ld_g + col);
     const L minus = spread<L>(-mean[row]), rr = spread<L>(rstd[row]);
     L m0 = spread<L>((A)0), m1 = m0;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(NormArgs a, const T* 
     }
     if (dx) store_vec<T, V>(dx + row * a.dim + col, o);
   }
-  A* out = part + (long long)blockIdx.x * 2 * a.dim;
+  A* out = part + (long long)blockIdx.y * 2 * a.dim;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (!(which ? a.want_db : a.want_dw)) continue;
@@ -242,7 +242,7 @@ cudaError_t norm_backward_rows(NormArgs a, const T* x, const T* g, const Acc<T>*
     if (dx) norm_means_kernel<T, P, V><<<norm_grid(a.rows, p, sms, 2), 1024, 0, st>>>(a, x, g, m, r, means);
     const int cols = (a.nv + 255) / 256, want = 4 * sms / cols > 1 ? 4 * sms / cols : 1;   // four blocks a SM
     *parts = (int)(a.rows < want ? a.rows : want);
-    norm_columns_kernel<T, P, V><<<dim3(*parts, cols), 256, 0, st>>>(a, x, g, m, r, means, dx, part);
+    norm_columns_kernel<T, P, V><<<dim3(cols, *parts), 256, 0, st>>>(a, x, g, m, r, means, dx, part);
     return cudaGetLastError();
   }
   if constexpr (std::is_same<P, T>::value) {

@@ -70,13 +70,27 @@ void check_status(int rc) {
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
+// Forward-mode derivatives would be lost without a word.
+void check_forward_mode(const char* what, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), what, " has no forward-mode derivative");
+}
+
+// t with its values in memory: not behind a pending negation (the imaginary part of
+// a conjugate), and not a zero tensor without storage.
+Tensor plain(const Tensor& t) {
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
 // t as rows of `dim` values with unit stride along the row; copied only where the
 // strides do not allow that.
 struct Rows {
   Tensor t;
   int64_t ld;
 };
-Rows as_rows(const Tensor& t, int64_t dim) {
+Rows as_rows(const Tensor& given, int64_t dim) {
+  const Tensor t = plain(given);
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, dim});
   const int64_t n = r.size(0);
   // (and rows 4 GiB apart and more, which the edge kernels do not address)
@@ -204,18 +218,19 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, const std::optio
     TORCH_CHECK_VALUE(scale->dim() == 1 && scale->size(0) == dim, "scale must have shape (", dim, ",), got ", scale->sizes());
     check_device("scale", *scale, "table", table);
     a.mode = LG_SCALE_COLUMN;
-    column = scale->contiguous();
+    column = plain(*scale).contiguous();
   } else if (has_value) {
     a.mode = LG_SCALE_VALUE;
     a.value = value;
   }
   a.has_pad = padding.has_value();
   a.pad = padding.value_or(0);
-  const Tensor at = ids.contiguous();
+  const Tensor at = plain(ids).contiguous();
+  check_forward_mode("embedding_lookup", {table, column});
   const bool differentiate = at::GradMode::is_enabled() && (wants_grad(table) || wants_grad(column));
   Tensor out;
   {
-    const at::AutoDispatchBelowADInplaceOrView plain;
+    const at::AutoDispatchBelowADInplaceOrView below;
     out = gather(table, column, at, a);
   }
   if (differentiate) {
@@ -313,14 +328,15 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
                      half ? " or torch.float32" : "", ", got ", name_of(p->scalar_type()));
     TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == dim, name, " must have shape (", dim, ",), got ", p->sizes());
     check_device(name, *p, "x", x);
-    (k ? b : w) = p->contiguous();
+    (k ? b : w) = plain(*p).contiguous();
   }
   TORCH_CHECK_TYPE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
                    "weight and bias must have the same type");
+  check_forward_mode("layer_norm", {x, w, b});
   const bool differentiate = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b));
   Tensor out, stats;
   {
-    const at::AutoDispatchBelowADInplaceOrView plain;
+    const at::AutoDispatchBelowADInplaceOrView below;
     out = norm_forward(x, w, b, eps, differentiate ? &stats : nullptr);
   }
   if (differentiate) {
@@ -373,7 +389,7 @@ c10::intrusive_ptr<EdgeGraph> edge_graph(const Tensor& given, int64_t n) {
   if (m == 0) return g;
   const c10::cuda::CUDAGuard guard(given.device());
   g->built_on = stream_of(given);
-  const Tensor idx = given.to(at::kLong).contiguous();
+  const Tensor idx = plain(given).to(at::kLong).contiguous();
   const auto i32 = idx.options().dtype(at::kInt);
   g->ends = at::empty({2 * m}, i32);
   g->rowptr = at::empty({n + 1}, i32);
@@ -436,7 +452,7 @@ struct EdgeDistBackward : public Node {
     if (e.m) {
       e.use();
       const Rows t = as_rows(v, dim);
-      const Tensor g = grads[0].contiguous();
+      const Tensor g = plain(grads[0]).contiguous();
       const int code = code_of(v.scalar_type());
       const size_t nb = lg_edge_sqdist_grad_workspace_bytes(e.n, e.m, (int)dim, code, t.t.data_ptr(), t.ld,
                                                              e.nlong ? (int)e.nchunks : 0);
@@ -456,10 +472,11 @@ Tensor edge_sqdist(const Tensor& x, const c10::intrusive_ptr<EdgeGraph>& g) {
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == g->n && x.size(1) >= 1 && x.size(1) <= (1 << 20), "x must be (", g->n,
                     ", dim), got shape ", x.sizes());
   TORCH_CHECK_VALUE(x.device() == g->device, "x is on ", x.device(), ", the edges on ", g->device);
+  check_forward_mode("EdgeDistances", {x});
   const bool differentiate = at::GradMode::is_enabled() && wants_grad(x);
   Tensor out;
   {
-    const at::AutoDispatchBelowADInplaceOrView plain;
+    const at::AutoDispatchBelowADInplaceOrView below;
     out = edge_forward(x, *g);
   }
   if (differentiate) {

@@ -21,8 +21,10 @@ in a fixed order, so equal inputs give equal bits.  Calls run on the current
 stream of their tensors' device, allocate from torch and wait for nothing
 (``EdgeDistances`` checks its indices when it is built, which waits once; the
 rest can be captured into CUDA graphs; as with torch's own operations, capture a
-backward pass only when no eager autograd graph of the same leaves is alive).  The gradients are not differentiable
-themselves (a second backward pass raises).  There is no CPU implementation.
+backward pass only when no eager autograd graph of the same leaves is alive).
+The gradients are not differentiable themselves (a second backward pass raises),
+and there are no forward-mode derivatives (NotImplementedError).  There is no
+CPU implementation.
 
 Squared distances are the ``x_edge_dists`` of
 ``gpu_eigsh.imgp.make_imgp_precision_matvec``.  That operator differentiates

@@ -516,6 +516,75 @@ def test_edges_strides_and_nonfinite():
     assert torch.equal(a, b)
 
 
+def test_values_behind_a_pending_negation():
+    """The imaginary part of a conjugate holds the negated values in memory."""
+    from gpu_eigsh.features import edge_sqdist, embedding_lookup, layer_norm
+
+    z = torch.complex(randn((40, 1), torch.float32, 1), randn((40, 1), torch.float32, 2))
+    neg = z.conj().imag
+    val = -z.imag
+    assert neg.is_neg() and not val.is_neg()
+    ids = make_ids("uniform", 40, 100, 3)
+    idx = make_edges(40, 60, 4)
+    assert torch.equal(embedding_lookup(neg, ids), val[ids])
+    assert torch.equal(edge_sqdist(neg + 0, idx), edge_sqdist(val, idx)) and torch.equal(edge_sqdist(neg, idx), edge_sqdist(val, idx))
+    x, w = randn((5, 40), torch.float32, 5), neg.reshape(40)
+    assert torch.equal(layer_norm(x, w), layer_norm(x, val.reshape(40)))
+    assert torch.equal(layer_norm(neg.T, None, w), layer_norm(val.T.contiguous(), None, val.reshape(40)))
+    s = torch._neg_view(randn((3,), torch.float32, 6))
+    W = randn((40, 3), torch.float32, 7)
+    assert torch.equal(embedding_lookup(W, ids, scale=s), embedding_lookup(W, ids, scale=s.clone()))
+    g = torch._neg_view(randn((100, 3), torch.float32, 8))
+    W.requires_grad_(True)
+    a, b = (torch.autograd.grad(embedding_lookup(W, ids), [W], h)[0] for h in (g, g.clone()))
+    assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+
+    from gpu_eigsh.features import edge_sqdist, embedding_lookup, layer_norm
+
+    x = randn((6, 4), torch.float32, 1)
+    ids = torch.arange(6, device="cuda")
+    with fwad.dual_level():
+        d = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: embedding_lookup(d, ids), lambda: layer_norm(d), lambda: edge_sqdist(d, torch.stack([ids, ids]))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_layer_norm_of_the_longest_rows():
+    """2^24 columns in 2-byte pieces (an odd address), with all gradients: every column
+    against the formula over the row's own statistics in 64 bits."""
+    from gpu_eigsh.features import layer_norm
+
+    n = 2 ** 24
+    x = randn((n + 1,), torch.bfloat16, 1)[1:].reshape(1, n).detach().requires_grad_(True)
+    w = randn((n,), torch.bfloat16, 2).requires_grad_(True)
+    g = randn((1, n), torch.bfloat16, 3)
+    y = layer_norm(x, w)
+    dx, dw = torch.autograd.grad(y, [x, w], g)
+    X, W, G = (t.detach().to(F64) for t in (x, w, g))
+    mu = X.mean()
+    r = 1 / torch.sqrt(((X - mu) ** 2).mean() + 1e-5)
+    h = (X - mu) * r
+    wg = W * G
+    ref = r * (wg - wg.mean() - h * (wg * h).mean())
+    # sums of 2^24 terms by 1024 threads (2^14 terms each, then a tree): under 2^14 + 32 roundings of
+    # 2^-24 relative to the sum of magnitudes, at most 2^-9.9 of mean |.| in a mean, and one rounding
+    # of 2^-8 relative to the result
+    off = 2.0 ** -9.9
+    err_mu = off * X.abs().mean()
+    err_h = (err_mu * r + h.abs() * 2 * off) * SLACK
+    check(y.detach(), h * W, err_h * W.abs() + 2.0 ** -8 * (h * W).abs() * SLACK + tiny(torch.bfloat16), "y")
+    check(dw[None], h * G, err_h * G.abs() + 2.0 ** -8 * (h * G).abs() * SLACK + tiny(torch.bfloat16), "dw")
+    m = (wg * h).mean().abs()
+    err = r * (off * wg.abs().mean() + err_h * (m + off * (wg * h).abs().mean()) +
+               h.abs() * (off * (wg * h).abs().mean() + (wg.abs() * err_h).mean())) + 3 * off * ref.abs()
+    check(dx, ref, err * SLACK + 2.0 ** -8 * ref.abs() * SLACK + tiny(torch.bfloat16), "dx")
+
+
 def test_edges_many():
     """The lists of a large graph, and their sort over several passes."""
     edge_case(torch.float32, 200000, 1000000, 4, seed=9)
