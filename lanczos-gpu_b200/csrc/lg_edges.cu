@@ -16,9 +16,9 @@
 // a group keeps several edges' rows in flight; by the sectors that they touch; and by
 // the instructions around them, so a lane takes two vectors of a row where the row
 // has more than two.  10^6 vertices, 5 10^6 edges with far ends, 10 fp32: forward
-// 84 us, backward 136 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
-// pieces take the same, and a lane a vector costs 240 us instead of 220.  10^5
-// vertices, 10^6 edges, 64 fp32: 95 us for both.
+// 67 us, backward 136 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
+// pieces take the same, and a lane a vector takes 20 us longer.  10^5
+// vertices, 10^6 edges, 64 fp32: 32 us and 53 us.
 #include "lg_feat.cuh"
 
 #include "../../include/lanczos_b200.h"
@@ -97,10 +97,19 @@ template <typename T> __device__ __forceinline__ const T* row_at(const T* x, int
 
 constexpr int kEdges = 4;
 
-// K vectors a lane; LOOP: the row has more than K << lg.
+// Blocks that an SM is to hold, which sets the registers: the most that do not spill
+// them.  10^6 vertices, 5 10^6 edges, 10 fp32 in pairs: 67 us with 6, 70 us with 5,
+// 80 us without a bound; 50,000 vertices, 500,000 edges, 1024 fp32: 250 us with 4,
+// 262 us with 3, 316 us without.
 template <typename T, int V, int K, bool LOOP>
-__global__ void __launch_bounds__(kThreads) edge_dist_kernel(EdgeArgs a, const int* __restrict__ ends,
-                                                             const T* __restrict__ x, Acc<T>* __restrict__ d2) {
+constexpr int dist_blocks = K == 1 ? 4 : sizeof(T) * V <= 8 ? 6 : sizeof(T) == 8 && LOOP ? 3 : 4;
+
+// K vectors a lane; LOOP: the row has more than K << lg.  All vectors of a turn are on
+// their way before the first is used (64 fp32, 10^6 edges: 35 us, 40 us one vector
+// after the other).
+template <typename T, int V, int K, bool LOOP>
+__global__ void __launch_bounds__(kThreads, dist_blocks<T, V, K, LOOP>)
+    edge_dist_kernel(EdgeArgs a, const int* __restrict__ ends, const T* __restrict__ x, Acc<T>* __restrict__ d2) {
   typedef Acc<T> A;
   typedef Lane<T, V> L;
   const int lane = threadIdx.x & ((1 << a.lg) - 1);
@@ -118,21 +127,28 @@ __global__ void __launch_bounds__(kThreads) edge_dist_kernel(EdgeArgs a, const i
   }
   const L minus = spread<L>((A)-1);
   for (int c = lane; c < (LOOP ? a.nv : lane + 1); c += K << a.lg) {
+    Vec<T, V> p[K][kEdges], q[K][kEdges];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (c + (k << a.lg) >= a.nv) break;
-      Vec<T, V> p[kEdges], q[kEdges];
       const int at = (c - lane + (k << a.lg)) * V;
 #pragma unroll
       for (int u = 0; u < kEdges; ++u) {
-        p[u] = load_vec<T, V>(xi[u] + at);
-        q[u] = load_vec<T, V>(xj[u] + at);
+        typename Word<sizeof(T) * V>::type zero = {};
+        memcpy(&p[k][u], &zero, sizeof(zero));
+        memcpy(&q[k][u], &zero, sizeof(zero));
+        if (c + (k << a.lg) < a.nv) {
+          p[k][u] = load_vec<T, V>(xi[u] + at);
+          q[k][u] = load_vec<T, V>(xj[u] + at);
+        }
       }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int u = 0; u < kEdges; ++u) {
 #pragma unroll
         for (int n = 0; n < lanes<V>; ++n) {
-          const L d = fma(widen<T, V>(q[u].v, n), minus, widen<T, V>(p[u].v, n));
+          const L d = fma(widen<T, V>(q[k][u].v, n), minus, widen<T, V>(p[k][u].v, n));
           s[u] = fma(d, d, s[u]);
         }
       }
