@@ -16,7 +16,7 @@
 // a group keeps several edges' rows in flight; by the sectors that they touch; and by
 // the instructions around them, so a lane takes two vectors of a row where the row
 // has more than two.  10^6 vertices, 5 10^6 edges with far ends, 10 fp32: forward
-// 67 us, backward 136 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
+// 67 us, backward 138 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
 // pieces take the same, and a lane a vector takes 20 us longer.  10^5
 // vertices, 10^6 edges, 64 fp32: 32 us and 53 us.
 #include "lg_feat.cuh"
