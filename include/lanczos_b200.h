@@ -488,8 +488,9 @@ int lg_outer_accumulate(int n, int dtype, const void* lam, const void* x, int ld
  * outputs are contiguous.  Arithmetic, sums and the parameters said to be in
  * the accumulation type are in fp64 for LG_F64, else in fp32; results are
  * rounded once.  Every call only enqueues work on `stream`; sums run in a fixed
- * order, so equal inputs give equal bits.  Addresses and strides may have any
- * alignment; multiples of 16 bytes are fastest. */
+ * order, so equal calls give equal bits.  Addresses are multiples of their
+ * element's size and those of workspaces of 16 bytes (else the call is refused);
+ * rows at multiples of 16 bytes are fastest. */
 
 /* out[t, :] = s * table[ids[t], :] for t < n (ids: int64, or int32 when ids64 =
  * 0).  scale_mode LG_SCALE_NONE, LG_SCALE_VALUE (s = scale_value) or

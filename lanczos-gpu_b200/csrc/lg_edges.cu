@@ -428,7 +428,8 @@ extern "C" size_t lg_edge_graph_workspace_bytes(long long n, long long m) {
 extern "C" int lg_edge_graph(long long n, long long m, const long long* idx, int* ends, int* rowptr, int* other,
                              int* eid, int* bad, void* ws, size_t ws_bytes, void* stream) {
   if (!edge_sizes_ok(n, m) || !idx || !ends || !rowptr || !other || !eid || !bad || !ws ||
-      ws_bytes < sort_ids_workspace(n, 2 * m))
+      ws_bytes < sort_ids_workspace(n, 2 * m) || !aligned(8, idx) || !aligned(4, ends, rowptr, other, eid, bad) ||
+      !aligned(kWsAlign, ws))
     return bad_args("lg_edge_graph: invalid arguments");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemsetAsync(bad, 0, sizeof(int), st);
@@ -454,7 +455,8 @@ extern "C" size_t lg_edge_sqdist_workspace_bytes(long long n, long long m, int d
 extern "C" int lg_edge_sqdist(long long n, long long m, int dim, int dtype, const int* ends, const void* x,
                               long long ld_x, void* d2, void* ws, size_t ws_bytes, void* stream) {
   const size_t nb = lg_edge_sqdist_workspace_bytes(n, m, dim, dtype, x, ld_x);
-  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !ends || !x || !d2 || (nb && (!ws || ws_bytes < nb)))
+  if (!edge_args_ok(n, m, dim, dtype, ld_x) || !ends || !x || !d2 || (nb && (!ws || ws_bytes < nb)) ||
+      !aligned(4, ends) || !aligned(elem_size(dtype), x) || !aligned(acc_size(dtype), d2) || !aligned(kWsAlign, ws))
     return bad_args("lg_edge_sqdist: invalid arguments");
   EdgeArgs a = {};
   a.n = n;
@@ -497,7 +499,9 @@ extern "C" int lg_edge_sqdist_grad(long long n, long long m, int dim, int dtype,
                                    const int* chunk_row, const int* chunk_first, const void* x, long long ld_x,
                                    const void* g, void* dx, void* ws, size_t ws_bytes, void* stream) {
   if (!edge_args_ok(n, m, dim, dtype, ld_x) || !rowptr || !other || !eid || !x || !g || !dx || nlong < 0 ||
-      nchunks < nlong || (nlong > 0 && (!long_row || !long_first || !chunk_row || !chunk_first)))
+      nchunks < nlong || (nlong > 0 && (!long_row || !long_first || !chunk_row || !chunk_first)) ||
+      !aligned(4, rowptr, other, eid, long_row, long_first, chunk_row, chunk_first) ||
+      !aligned(elem_size(dtype), x, dx) || !aligned(acc_size(dtype), g) || !aligned(kWsAlign, ws))
     return bad_args("lg_edge_sqdist_grad: invalid arguments");
   if (nlong == 0) nchunks = 0;
   const size_t nb = lg_edge_sqdist_grad_workspace_bytes(n, m, dim, dtype, x, ld_x, nchunks);

@@ -204,6 +204,13 @@ struct Align {
   }
 };
 
+// Whether every address (null allowed) is a multiple of `bytes`: one that is not
+// would be a misaligned access on the device.
+template <typename... P> inline bool aligned(size_t bytes, const P*... p) {
+  return (... && (reinterpret_cast<uintptr_t>(p) % bytes == 0));
+}
+constexpr size_t kWsAlign = 16;   // of a workspace
+
 inline int sm_count() {
   static std::atomic<int> cache[64] = {};
   int dev = 0;

@@ -288,7 +288,9 @@ extern "C" int lg_layer_norm_backward(long long rows, int dim, int dtype, const 
                                       const void* rstd, void* dx, void* d_weight, void* d_bias, void* ws,
                                       size_t ws_bytes, void* stream) {
   if (!norm_args_ok(rows, dim, dtype, param_dtype) || !x || !g || ld_x < dim || ld_g < dim || !mean || !rstd ||
-      (!dx && !d_weight && !d_bias) || !ws)
+      (!dx && !d_weight && !d_bias) || !ws || !aligned(elem_size(dtype), x, g, dx) ||
+      !aligned(elem_size(param_dtype), weight, d_weight, d_bias) || !aligned(acc_size(dtype), mean, rstd) ||
+      !aligned(kWsAlign, ws))
     return bad_args("lg_layer_norm_backward: invalid arguments");
   const int sms = sm_count();
   if (sms < 1) return bad_args("lg_layer_norm_backward: no CUDA device");

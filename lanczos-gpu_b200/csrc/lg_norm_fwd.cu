@@ -189,7 +189,8 @@ extern "C" int lg_layer_norm_forward(long long rows, int dim, int dtype, const v
                                      const void* weight, const void* bias, double eps, void* y, void* mean, void* rstd,
                                      void* stream) {
   if (!norm_args_ok(rows, dim, dtype, param_dtype) || !x || !y || ld_x < dim || !(eps >= 0.0) ||
-      (mean == nullptr) != (rstd == nullptr))
+      (mean == nullptr) != (rstd == nullptr) || !aligned(elem_size(dtype), x, y) ||
+      !aligned(elem_size(param_dtype), weight, bias) || !aligned(acc_size(dtype), mean, rstd))
     return bad_args("lg_layer_norm_forward: invalid arguments");
   const int sms = sm_count();
   if (sms < 1) return bad_args("lg_layer_norm_forward: no CUDA device");

@@ -965,7 +965,8 @@ using namespace lg::feat;
 extern "C" int lg_rows_gather(long long rows, int dim, int dtype, const void* table, long long ld_table, long long n,
                               const void* ids, int ids64, int scale_mode, const void* scale, double scale_value,
                               int has_padding, long long padding, void* out, void* stream) {
-  if (!rows_args_ok(rows, dim, dtype, n, ids, scale_mode, scale) || !table || !out || ld_table < dim)
+  if (!rows_args_ok(rows, dim, dtype, n, ids, scale_mode, scale) || !table || !out || ld_table < dim ||
+      !aligned(elem_size(dtype), table, out) || !aligned(ids64 ? 8 : 4, ids) || !aligned(acc_size(dtype), scale))
     return bad_args("lg_rows_gather: invalid arguments");
   GatherArgs a = {};
   a.rows = rows;
@@ -1002,7 +1003,8 @@ extern "C" int lg_rows_scatter(long long rows, int dim, int dtype, const void* t
                                int has_padding, long long padding, const void* g, long long ld_g, void* d_table,
                                void* d_scale, void* ws, size_t ws_bytes, void* stream) {
   if (!rows_args_ok(rows, dim, dtype, n, ids, scale_mode, scale) || !g || ld_g < dim || !ws || (!d_table && !d_scale) ||
-      (d_scale && (!table || ld_table < dim || scale_mode != kColumn)))
+      (d_scale && (!table || ld_table < dim || scale_mode != kColumn)) || !aligned(elem_size(dtype), table, g, d_table) ||
+      !aligned(acc_size(dtype), scale, d_scale) || !aligned(ids64 ? 8 : 4, ids) || !aligned(kWsAlign, ws))
     return bad_args("lg_rows_scatter: invalid arguments");
   const ScatterLayout l = scatter_layout(rows, dim, dtype, n, d_scale != nullptr);
   if (ws_bytes < l.total) return bad_args("lg_rows_scatter: workspace too small");

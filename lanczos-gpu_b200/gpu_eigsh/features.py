@@ -17,7 +17,8 @@ as torch functions of CUDA tensors:
 
 Element types: float32, float64, float16 and bfloat16.  Arithmetic and sums
 are in float32 (float64 for float64), each result is rounded once.  Sums run
-in a fixed order, so equal inputs give equal bits.  Calls run on the current
+in a fixed order, so equal calls give equal bits (an order may depend on the
+strides and the alignment of the inputs).  Calls run on the current
 stream of their tensors' device, allocate from torch and wait for nothing
 (``EdgeDistances`` checks its indices when it is built, which waits once; the
 rest can be captured into CUDA graphs; as with torch's own operations, capture a
@@ -109,7 +110,7 @@ class EdgeDistances:
     gradients to x.  Building it sorts the edge ends, checks the indices
     (ValueError; one wait for the device) and keeps 24 bytes an edge; any number
     of calls may use it at once, on any stream that has waited for the one it
-    was built on.
+    was built on.  Keep it as long as a captured CUDA graph that uses it.
     """
 
     def __init__(self, idx, n: int):

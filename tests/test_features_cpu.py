@@ -77,6 +77,32 @@ def test_norm_backward_refuses(bad):
     assert "lg_layer_norm_backward" in _native.last_error()
 
 
+def test_misaligned_addresses_are_refused():
+    """An address inside an element would be a fault on the device."""
+    for bad in (dict(table=P + 2), dict(out=P + 2), dict(ids=P + 4), dict(mode=2, scale=P + 2), dict(dtype=1, table=P + 4),
+                dict(dtype=3, out=P + 1), dict(dtype=1, mode=2, scale=P + 4)):
+        assert gather(**bad) == BAD, bad
+    for bad in (dict(ids=P + 4), dict(g=P + 2), dict(dw=P + 2), dict(ws=P + 8), dict(mode=2, scale=P, ds=P + 2),
+                dict(mode=2, scale=P, ds=P, table=P + 2)):
+        assert scatter(**bad) == BAD, bad
+    for bad in (dict(x=P + 2), dict(y=P + 1), dict(mean=P + 2, rstd=P), dict(dtype=1, pd=1, mean=P, rstd=P + 4)):
+        assert norm_fwd(**bad) == BAD, bad
+    big = 1 << 30
+
+    def norm_bwd(x=P, g=P, mean=P, dx=P, dw=None, ws=P):
+        return L.lg_layer_norm_backward(4, 3, 0, x, 3, g, 3, 0, None, mean, P, dx, dw, None, ws, big, None)
+
+    for bad in (dict(x=P + 2), dict(g=P + 1), dict(mean=P + 2), dict(dx=P + 2), dict(dw=P + 2), dict(ws=P + 8)):
+        assert norm_bwd(**bad) == BAD, bad
+    assert L.lg_edge_graph(4, 4, P + 4, P, P, P, P, P, P, big, None) == BAD
+    assert L.lg_edge_graph(4, 4, P, P + 2, P, P, P, P, P, big, None) == BAD
+    assert L.lg_edge_graph(4, 4, P, P, P, P, P, P, P + 8, big, None) == BAD
+    for ends, x, d2 in ((P + 2, P, P), (P, P + 2, P), (P, P, P + 2)):
+        assert L.lg_edge_sqdist(4, 4, 3, 0, ends, x, 3, d2, None, 0, None) == BAD
+    for x, g, dx, ws in ((P + 2, P, P, P), (P, P + 2, P, P), (P, P, P + 2, P), (P, P, P, P + 8)):
+        assert L.lg_edge_sqdist_grad(4, 4, 3, 0, P, P, P, 0, None, None, 0, None, None, x, 3, g, dx, ws, big, None) == BAD
+
+
 def test_edge_calls_refuse():
     big = 1 << 30
     assert L.lg_edge_graph_workspace_bytes(0, 4) == 0 and L.lg_edge_graph_workspace_bytes(4, 0) == 0
