@@ -151,6 +151,13 @@ def test_lookup_runs_at_tile_borders(n):
         lookup_case(torch.float32, rows, 6, n, kind, "column", seed=n)
 
 
+@pytest.mark.parametrize("n", [1, 4095, 4096, 4097, 4128, 4129])
+@pytest.mark.parametrize("dim", [510, 512, 513])
+def test_column_scale_gradient_by_the_last_block_or_a_launch(n, dim):
+    """Up to 128 blocks of 32 sorted ids a column piece add up the scale's gradient themselves."""
+    lookup_case(torch.float32, 3000, dim, n, "zipf", "column", pad=1, seed=n)
+
+
 @pytest.mark.parametrize("n,kind", [(3, "uniform"), (700, "zipf"), (5000, "zipf"), (20000, "uniform"), (40000, "zipf"),
                                     (140000, "zipf")])
 def test_lookup_large_tables(n, kind):
