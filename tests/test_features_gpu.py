@@ -131,6 +131,14 @@ def test_lookup(dt, rows, dim, n, kind, scale):
     lookup_case(DT[dt], rows, dim, n, kind, scale)
 
 
+@pytest.mark.parametrize("dt", sorted(DT))
+@pytest.mark.parametrize("dim", [3, 5, 6, 7, 9, 17, 25, 26, 27, 33, 47, 48, 49, 100, 132, 192, 196, 384, 392])
+def test_lookup_rows_that_leave_lanes_idle(dim, dt):
+    """Row lengths on both sides of the choice between a group of lanes a row and all vectors in one line."""
+    for n in (1, 341, 1025):
+        lookup_case(DT[dt], 60, dim, n, "uniform", "column" if n == 341 else "none", pad=5, out_of_range=True, seed=dim)
+
+
 @pytest.mark.parametrize("pad", [-1, 0, 6, 49, 10 ** 12])
 @pytest.mark.parametrize("scale", ["none", "column"])
 def test_lookup_padding_and_out_of_range(pad, scale):
