@@ -13,12 +13,12 @@
 // rest.
 //
 // Both directions are bound by the gathers of x rows from L2: by their latency, so
-// a group keeps several edges' rows in flight; by the sectors that they touch; and by
-// the instructions around them, so a lane takes two vectors of a row where the row
-// has more than two.  10^6 vertices, 5 10^6 edges with far ends, 10 fp32: forward
-// 67 us, backward 138 us (0.95 GB of L2 sectors: 7 TB/s); rows of 12 in 16-byte
-// pieces take the same, and a lane a vector takes 20 us longer.  10^5
-// vertices, 10^6 edges, 64 fp32: 32 us and 53 us.
+// a group keeps several edges' rows in flight; by L1, which looks up every row a lane
+// group touches; and by the instructions around them, so a lane takes two vectors of a
+// row where the row has more than two.  10^6 vertices, 5 10^6 edges with far ends, 10
+// fp32: forward 67 us (L1 71 % busy, 68 % of the issue slots), backward 138 us (80 %,
+// 56 %); rows of 12 in 16-byte pieces take the same, and a lane a vector takes 20 us
+// longer.  10^5 vertices, 10^6 edges, 64 fp32: 32 us and 53 us.
 #include "lg_feat.cuh"
 
 #include "../../include/lanczos_b200.h"
