@@ -45,13 +45,28 @@ def _device_points(points) -> torch.Tensor:
     return points.to(dev, torch.float64).contiguous()
 
 
+# Added to the variance of a normalised point.  Spreads below are at least 1, so
+# variances at least 1 / (2 dim): it changes them by at most 2e-12 dim of themselves.
+_NORM_EPS = 1e-12
+
+
 def _normalized(points) -> torch.Tensor:
     """Every point with mean 0 and variance 1 over its coordinates
-    (gpu_eigsh.features.layer_norm in fp64)."""
+    (gpu_eigsh.features.layer_norm in fp64), whatever the points' units: a point
+    whose spread lies outside [1, 2^16) is first multiplied by the power of 2^16
+    that brings it there, which rounds nothing."""
     P = _device_points(points)
     if P.shape[1] < 2:
         raise ValueError("normalize needs points of at least two coordinates")
-    return layer_norm(P, eps=1e-12)
+    lo, hi = torch.aminmax(P, dim=1)
+    flat = lo == hi
+    if bool(flat.any()):
+        raise ValueError(f"point {int(flat.nonzero()[0])} has equal coordinates: it has no correlation with others")
+    # spread = m 2^e, 1/2 <= m < 1; the factor 2^-shift as two powers of two within fp64's range
+    _, e = torch.frexp((hi - lo).clamp(max=torch.finfo(torch.float64).max))
+    shift = torch.div(e.to(torch.int64) - 1, 16, rounding_mode="floor") * 16
+    half = ((1023 - shift // 2) << 52).view(torch.float64)[:, None]
+    return layer_norm(P * half * half, eps=_NORM_EPS)
 
 
 def knn(points, k: int, method: str = "auto", normalize: bool = False):
@@ -62,7 +77,9 @@ def knn(points, k: int, method: str = "auto", normalize: bool = False):
     else all pairs), "cells" or "brute".
 
     normalize: layer-normalise every point first, so that neighbours are by
-    correlation: d2 = 2 dim (1 - correlation of the two points' coordinates)."""
+    correlation: d2 = 2 dim (1 - correlation of the two points' coordinates),
+    which does not depend on the points' units.  A point of equal coordinates
+    has no correlation (ValueError)."""
     if method not in _native.KNN_METHODS:
         raise ValueError(f"method must be one of {sorted(_native.KNN_METHODS)}")
     P = _normalized(points) if normalize else _device_points(points)
