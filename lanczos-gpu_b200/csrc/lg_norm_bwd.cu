@@ -32,7 +32,6 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_backward_kernel(
   __shared__ A red[BLOCK || !AFFINE ? 1 : 8][BLOCK || !AFFINE ? 1 : 32 * K * V];
   int half = 0;
   const Team<BLOCK> t(a.lg);
-  const A inv = (A)1 / (A)a.dim;
   Params<P, V> w[K];
   L dw[K][N], db[K][N];
 #pragma unroll
@@ -76,7 +75,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_backward_kernel(
     if (!dx) continue;
     A s[2] = {sum(s0), sum(s1)};
     team_sum<A, 2, BLOCK>(s, a.lg, scratch, half);
-    const L m0 = spread<L>(-(s[0] * inv)), m1 = spread<L>(-(s[1] * inv));
+    const L m0 = spread<L>(-mean_of(s[0], a)), m1 = spread<L>(-about_mean(s[1], a));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (on && rows.in[k]) {
@@ -144,7 +143,6 @@ __global__ void __launch_bounds__(1024) norm_means_kernel(NormArgs a, const T* _
   __shared__ __align__(16) A scratch[128];
   clear_scratch(scratch, 128);
   int half = 0;
-  const A inv = (A)1 / (A)a.dim;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* px = x + row * a.ld_x;
     const T* pg = g + row * a.ld_g;
@@ -164,8 +162,8 @@ __global__ void __launch_bounds__(1024) norm_means_kernel(NormArgs a, const T* _
     A s[2] = {sum(s0), sum(s1)};
     team_sum<A, 2, true>(s, 0, scratch, half);
     if (threadIdx.x == 0) {
-      means[2 * row] = s[0] * inv;
-      means[2 * row + 1] = s[1] * inv;
+      means[2 * row] = mean_of(s[0], a);
+      means[2 * row + 1] = about_mean(s[1], a);
     }
   }
 }
@@ -298,7 +296,7 @@ extern "C" int lg_layer_norm_backward(long long rows, int dim, int dtype, const 
     return bad_args("lg_layer_norm_backward: workspace too small");
   NormArgs a = {};
   a.rows = rows;
-  a.dim = dim;
+  set_dim(a, dim);
   a.ld_x = ld_x;
   a.ld_g = ld_g;
   a.w = weight;

@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_forward_kernel(Norm
   if (BLOCK) clear_scratch(scratch, 64);
   int half = 0;
   const Team<BLOCK> t(a.lg);
-  const A inv = (A)1 / (A)a.dim;
+  const A count = (A)a.dim, inv = (A)1 / count;
   constexpr bool kept = K <= 4;   // weight and bias stay in registers; else they are read again (from L1) for every row
   Params<P, V> w[kept ? K : 1], b[kept ? K : 1];
   if (kept && AFFINE) {
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlock : 256) norm_forward_kernel(Norm
     }
     s[0] = sum(acc);
     team_sum<A, 1, BLOCK>(s, a.lg, scratch, half);
-    const A mu = s[0] * inv;
+    const A mu = mean_of(s[0], count, inv);
     const L minus = spread<L>(-mu);
     acc = spread<L>((A)0);
 #pragma unroll
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(1024) norm_forward_long_kernel(NormArgs a, con
   __shared__ __align__(16) A scratch[64];
   clear_scratch(scratch, 64);
   int half = 0;
-  const A inv = (A)1 / (A)a.dim;
+  const A count = (A)a.dim, inv = (A)1 / count;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* p = x + row * a.ld_x;
     A s[1] = {0};
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(1024) norm_forward_long_kernel(NormArgs a, con
       for (int i = 0; i < V; ++i) s[0] += to_acc(v.v[i]);
     }
     team_sum<A, 1, true>(s, 0, scratch, half);
-    const A mu = s[0] * inv;
+    const A mu = mean_of(s[0], count, inv);
     s[0] = 0;
     for (int c = threadIdx.x; c < a.nv; c += 1024) {
       const Vec<T, V> v = load_vec<T, V>(p + (long long)c * V);
@@ -196,7 +196,7 @@ extern "C" int lg_layer_norm_forward(long long rows, int dim, int dtype, const v
   if (sms < 1) return bad_args("lg_layer_norm_forward: no CUDA device");
   NormArgs a = {};
   a.rows = rows;
-  a.dim = dim;
+  set_dim(a, dim);
   a.ld_x = ld_x;
   a.eps = eps;
   a.w = weight;
