@@ -36,7 +36,7 @@ import numpy as np
 import torch
 
 from . import _native
-from .features import embedding_lookup
+from .ordering import renumber_rows
 
 __all__ = ["differentiable_eigsh"]
 
@@ -96,7 +96,7 @@ class _DifferentiableEigsh(torch.autograd.Function):
         ctx.perm, ctx.order = perm, order
         ctx.n, ctx.k, ctx.cg = int(n), int(k), (int(cg_max_iters), float(cg_tol))
         ctx.vdev, ctx.vdtype = values.device, values.dtype
-        Yc = Y if pos is None else embedding_lookup(Y, pos)   # rows back in the caller's numbering
+        Yc = Y if pos is None else renumber_rows(Y, pos)   # rows back in the caller's numbering
         return evals.to(values.device), Yc.to(values.device)
 
     @staticmethod
@@ -107,7 +107,7 @@ class _DifferentiableEigsh(torch.autograd.Function):
         ge = None if g_evals is None else g_evals.detach().to(dev, torch.float64).contiguous()
         gv = None if g_evecs is None else g_evecs.detach().to(dev, torch.float64)
         if gv is not None and ctx.perm is not None:
-            gv = embedding_lookup(gv, ctx.perm)   # into the solve's numbering
+            gv = renumber_rows(gv, ctx.perm)   # into the solve's numbering
         gv = None if gv is None else gv.contiguous()
         grad = torch.empty(va.numel(), dtype=torch.float64, device=dev)
         iters = (C.c_int * k)()

@@ -35,7 +35,7 @@ import math
 import torch
 
 from . import _native, _slq
-from .features import embedding_lookup
+from .ordering import renumber_rows
 
 __all__ = ["make_imgp_precision_matvec", "ImgpPrecisionMatvec", "_matmul_symmetric_laplacian",
            "imgp_neg_marginal_log_likelihood"]
@@ -45,13 +45,6 @@ _MAXB = 128
 
 def _scalar(t) -> float:
     return float(t.detach().reshape(-1)[0]) if torch.is_tensor(t) else float(t)
-
-
-def _rows(X: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
-    """X[at] for an (n, B) block: the library's row lookup."""
-    if X.dim() == 2 and X.numel() and X.dtype in (torch.float32, torch.float64):
-        return embedding_lookup(X, at)
-    return X.index_select(0, at)
 
 
 class ImgpPrecisionMatvec:
@@ -117,10 +110,17 @@ class ImgpPrecisionMatvec:
 
     def to_internal(self, X: torch.Tensor) -> torch.Tensor:
         """Rows of X (caller's vertex order) in the operator's row order."""
-        return X if self.perm is None else _rows(X, self.perm)
+        return X if self.perm is None else X.index_select(0, self.perm)
 
     def to_caller(self, Y: torch.Tensor) -> torch.Tensor:
-        return Y if self.pos is None else _rows(Y, self.pos)
+        return Y if self.pos is None else Y.index_select(0, self.pos)
+
+    # the same for blocks that no derivative passes through
+    def _internal_block(self, X: torch.Tensor) -> torch.Tensor:
+        return X if self.perm is None else renumber_rows(X, self.perm)
+
+    def _caller_block(self, Y: torch.Tensor) -> torch.Tensor:
+        return Y if self.pos is None else renumber_rows(Y, self.pos)
 
     # -- L_sym(kappa) and dL/dkappa -----------------------------------------------
     def laplacian(self, kappa: float):
@@ -176,9 +176,9 @@ class _PrecisionApply(torch.autograd.Function):
         X2 = rhs.reshape(-1, 1) if rhs.dim() == 1 else rhs
         if X2.shape[0] != mv.n:
             raise ValueError(f"rhs has {X2.shape[0]} rows, the operator {mv.n}")
-        parts = _blocked(mv.to_internal(X2.detach().to(mv.device, mv.dtype)), mv.device, mv.dtype)
+        parts = _blocked(mv._internal_block(X2.detach().to(mv.device, mv.dtype)), mv.device, mv.dtype)
         outs = [op.apply(blk, b, blk.shape[1])[:, :b] for blk, b in parts]
-        Y = mv.to_caller(torch.cat(outs, dim=1) if len(outs) > 1 else outs[0])
+        Y = mv._caller_block(torch.cat(outs, dim=1) if len(outs) > 1 else outs[0])
         ctx.mv, ctx.ell, ctx.kap, ctx.shape = mv, ell, kap, rhs.shape
         ctx.rhs_dev, ctx.rhs_dtype = rhs.device, rhs.dtype
         ctx.parts = parts
@@ -195,13 +195,13 @@ class _PrecisionApply(torch.autograd.Function):
         mv = ctx.mv
         op = mv.operator(ctx.ell, ctx.kap)
         G2 = g.reshape(-1, 1) if g.dim() == 1 else g
-        gparts = _blocked(mv.to_internal(G2.detach().to(mv.device, mv.dtype)), mv.device, mv.dtype)
+        gparts = _blocked(mv._internal_block(G2.detach().to(mv.device, mv.dtype)), mv.device, mv.dtype)
         gxs, gp = [], torch.zeros(2, dtype=torch.float64, device=mv.device)
         for (blk, b), (gblk, _) in zip(ctx.parts, gparts):
             gX, gpp = op.apply_vjp(blk, gblk, b, blk.shape[1])
             gxs.append(gX[:, :b])
             gp = gp + gpp
-        g_rhs = mv.to_caller(torch.cat(gxs, dim=1) if len(gxs) > 1 else gxs[0])
+        g_rhs = mv._caller_block(torch.cat(gxs, dim=1) if len(gxs) > 1 else gxs[0])
         g_rhs = g_rhs.reshape(ctx.shape).to(ctx.rhs_dev, ctx.rhs_dtype)
         g_ell = gp[1] * mv.shift_derivative(ctx.ell)
         g_kap = gp[0]
@@ -257,7 +257,7 @@ class ImgpSLQEngine:
         mv = self.mv
         op = mv.operator(self.ell, self.kap)
         q_all, saved = [], []
-        for blk, b in _blocked(mv.to_internal(Z), mv.device, mv.dtype):
+        for blk, b in _blocked(mv._internal_block(Z.detach()), mv.device, mv.dtype):
             ld = blk.shape[1]
             V, Y, alpha, beta, znorm = op.forward(blk, b, ld, self.m)
             q, ga, gb, _ = _slq.small_side(alpha, beta, znorm, "log", 0, g_scale=1.0 / p_total)
