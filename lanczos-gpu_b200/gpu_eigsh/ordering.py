@@ -135,9 +135,10 @@ def permute_symmetric(rowptr: torch.Tensor, col: torch.Tensor, val: torch.Tensor
 def renumber_rows(X: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
     """X[at] of an (n, B) block that no derivative passes through (a detached
     tensor), by the library's row lookup: 10^6 x 64 fp32 in 88 us where
-    index_select takes 521, 10^5 x 20 fp64 in 6 where it takes 55.  Other types
-    and shapes are index_select's."""
-    if (X.dim() == 2 and X.shape[0] and 1 <= X.shape[1] <= 1 << 20 and X.is_cuda
+    index_select takes 521, 10^5 x 20 fp64 in 6 where it takes 55.  Single
+    columns are index_select's (10^6 fp32: 8.3 us, 9.6 by the lookup), as are
+    other types and shapes."""
+    if (X.dim() == 2 and X.shape[0] and 1 < X.shape[1] <= 1 << 20 and X.is_cuda
             and X.dtype in (torch.float32, torch.float64)):
         from .features import embedding_lookup
 
