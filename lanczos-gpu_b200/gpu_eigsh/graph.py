@@ -27,7 +27,6 @@ import numpy as np
 import torch
 
 from . import _native
-from .features import layer_norm
 
 __all__ = ["knn", "knn_laplacian", "generate_points", "generate_knn_laplacian"]
 
@@ -55,6 +54,8 @@ def _normalized(points) -> torch.Tensor:
     (gpu_eigsh.features.layer_norm in fp64), whatever the points' units: a point
     whose spread lies outside [1, 2^16) is first multiplied by the power of 2^16
     that brings it there, which rounds nothing."""
+    from .features import layer_norm
+
     P = _device_points(points)
     if P.shape[1] < 2:
         raise ValueError("normalize needs points of at least two coordinates")
