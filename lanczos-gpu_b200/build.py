@@ -9,12 +9,14 @@ library carries no dependency beyond the driver.  Objects go to _build/.
 Then csrc/torch/features.cpp, the torch binding of the node-feature operators,
 is compiled by g++ against the installed torch and that library into
 gpu_eigsh/_lib/_torch_features.so.  Rebuilds only what changed (any header
-change rebuilds everything).
+change rebuilds everything; the binding also for another torch, Python, compiler
+or compile command, which _torch_features.json beside it names).
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import json
 import os
 import shutil
 import subprocess
@@ -28,6 +30,7 @@ OUT_DIR = PKG / "gpu_eigsh" / "_lib"
 LIB = OUT_DIR / "liblanczos_b200.so"
 TORCH_SRC = CSRC / "torch" / "features.cpp"
 TORCH_LIB = OUT_DIR / "_torch_features.so"
+TORCH_STAMP = OUT_DIR / "_torch_features.json"   # what the binding was built for
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -69,6 +72,34 @@ def torch_binding_command() -> list[str]:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
             str(TORCH_SRC), "-o", str(TORCH_LIB), *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch",
             "-ltorch_cpu", "-ltorch_python", f"-L{OUT_DIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+
+
+def torch_binding_stamp(cmd: list[str]) -> str:
+    """What the binding depends on beside its sources: torch's C++ interface changes
+    between versions, and a binding for another one does not load, or runs on
+    objects of another layout."""
+    import sysconfig
+
+    import torch
+
+    compiler = subprocess.run([cmd[0], "--version"], capture_output=True, text=True).stdout.partition("\n")[0]
+    return json.dumps({"torch": torch.__version__, "python": sysconfig.get_config_var("SOABI"), "compiler": compiler,
+                       "command": [a.replace(str(PKG.parent), ".") for a in cmd]}, indent=1)
+
+
+def build_torch_binding(force: bool = False, verbose: bool = False) -> None:
+    cmd = torch_binding_command()
+    stamp = torch_binding_stamp(cmd)
+    if (not force and TORCH_LIB.exists() and TORCH_STAMP.exists() and TORCH_STAMP.read_text() == stamp
+            and TORCH_LIB.stat().st_mtime >= _newest([TORCH_SRC, *INCLUDE.glob("*.h")])):
+        return
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed for csrc/torch/features.cpp")
+    TORCH_STAMP.write_text(stamp)
 
 
 def _newest(paths) -> float:
@@ -118,14 +149,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
 
-    if force or not TORCH_LIB.exists() or TORCH_LIB.stat().st_mtime < _newest([TORCH_SRC, *INCLUDE.glob("*.h")]):
-        cmd = torch_binding_command()
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
-            raise RuntimeError("g++ failed for csrc/torch/features.cpp")
+    build_torch_binding(force, verbose)
     return LIB
 
 

@@ -40,6 +40,7 @@ many times a step on small inputs.
 from __future__ import annotations
 
 import importlib.util
+import json
 import operator
 from pathlib import Path
 
@@ -50,14 +51,23 @@ from . import _native  # noqa: F401  (loads liblanczos_b200.so, which the bindin
 __all__ = ["embedding_lookup", "layer_norm", "EdgeDistances", "edge_sqdist"]
 
 
-def _load():
-    path = Path(__file__).resolve().parent / "_lib" / "_torch_features.so"
+_BUILD = "build it with `python lanczos-gpu_b200/build.py`.  There is no Python fallback."
+
+
+def _load(path=Path(__file__).resolve().parent / "_lib" / "_torch_features.so"):
     if not path.exists():
-        raise ImportError(f"{path} is missing; build it with `python lanczos-gpu_b200/build.py`.  "
-                          "There is no Python fallback.")
-    spec = importlib.util.spec_from_file_location("_torch_features", path)
-    mod = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(mod)
+        raise ImportError(f"{path} is missing; {_BUILD}")
+    built_for = path.with_suffix(".json")
+    if built_for.exists():
+        version = json.loads(built_for.read_text())["torch"]
+        if version != torch.__version__:
+            raise ImportError(f"{path} was built for torch {version}, this is {torch.__version__}; {_BUILD}")
+    try:
+        spec = importlib.util.spec_from_file_location("_torch_features", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+    except ImportError as e:
+        raise ImportError(f"{path} does not load ({e}); {_BUILD}") from e
     return mod
 
 

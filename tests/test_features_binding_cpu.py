@@ -1,7 +1,12 @@
 """CPU: what depends on the compiled torch binding of the node features, and when it is built again."""
+import importlib.util
+import json
+import os
 import subprocess
 import sys
 from pathlib import Path
+
+import pytest
 
 PKG = Path(__file__).resolve().parents[1] / "lanczos-gpu_b200"
 
@@ -18,3 +23,62 @@ def test_other_modules_import_without_the_binding():
                  "import gpu_eigsh.ordering, gpu_eigsh.funm_torch, gpu_eigsh.distributed\n"
                  "from gpu_eigsh import differentiable_eigsh\n")
     assert res.returncode == 0, res.stderr
+
+
+@pytest.fixture()
+def build(tmp_path, monkeypatch):
+    """build.py with a binding in tmp_path whose compilation adds a byte to it."""
+    spec = importlib.util.spec_from_file_location("_build_under_test", PKG / "build.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    lib = tmp_path / "_torch_features.so"
+    mod.TORCH_LIB, mod.TORCH_STAMP = lib, tmp_path / "_torch_features.json"
+    mod.torch_binding_command = lambda: [sys.executable, "-c", f"open({str(lib)!r}, 'a').write('x')"]
+    mod.runs = lambda: lib.stat().st_size
+    return mod
+
+
+def test_binding_is_built_again_when_torch_changes(build):
+    build.build_torch_binding()
+    build.build_torch_binding()
+    assert build.runs() == 1
+    stamp = build.TORCH_STAMP.read_text()
+    for k, change in enumerate(("torch", "python", "compiler", "command")):
+        build.TORCH_STAMP.write_text(json.dumps({**json.loads(stamp), change: "another"}, indent=1))
+        build.build_torch_binding()
+        assert build.runs() == 2 + k and build.TORCH_STAMP.read_text() == stamp, change
+        build.build_torch_binding()
+        assert build.runs() == 2 + k
+    build.TORCH_STAMP.unlink()
+    build.build_torch_binding()
+    assert build.runs() == 6
+    os.utime(build.TORCH_LIB, (1, 1))   # older than the sources
+    build.build_torch_binding()
+    assert build.runs() == 7
+    build.build_torch_binding(force=True)
+    assert build.runs() == 8
+
+
+def test_a_failed_build_is_tried_again(build):
+    good = build.torch_binding_command
+    build.build_torch_binding()
+    build.torch_binding_command = lambda: [sys.executable, "-c", "raise SystemExit(3)"]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="features.cpp"):
+            build.build_torch_binding()
+    build.torch_binding_command = good
+    assert build.runs() == 1
+
+
+def test_a_binding_for_another_torch_is_refused(tmp_path):
+    from gpu_eigsh import features
+
+    lib = tmp_path / "_torch_features.so"
+    with pytest.raises(ImportError, match="missing; build it"):
+        features._load(lib)
+    lib.write_text("not a library")
+    with pytest.raises(ImportError, match="does not load"):
+        features._load(lib)
+    lib.with_suffix(".json").write_text(json.dumps({"torch": "1.0"}))
+    with pytest.raises(ImportError, match="built for torch 1.0, this is"):
+        features._load(lib)
