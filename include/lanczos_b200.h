@@ -533,7 +533,7 @@ int lg_layer_norm_backward(long long rows, int dim, int dtype, const void* x, lo
  * for every vertex the list of its edges (rowptr n + 1; other: the vertex at
  * the other end; eid: the edge), the edges it begins before those it ends,
  * ascending.  *bad (device int) becomes 1 if an index is outside [0, n); the
- * lists are then not to be used.  2m < 2^31 - 1. */
+ * lists are then not to be used.  2m <= 2^31 - 1 - LG_EDGE_CHUNK. */
 #define LG_EDGE_CHUNK 128
 size_t lg_edge_graph_workspace_bytes(long long n, long long m);
 int lg_edge_graph(long long n, long long m, const long long* idx, int* ends, int* rowptr, int* other, int* eid,

@@ -351,8 +351,10 @@ cudaError_t edge_grad(GradArgs a, int dim, const T* x, const void* g, T* dx, con
   return e;
 }
 
+// The gradient forms list positions a few beyond a list's end, and a list's length
+// rounded up to chunks, in 32 bits.
 bool edge_sizes_ok(long long n, long long m) {
-  return n >= 1 && n < 2147483647LL && m >= 1 && 2 * m < 2147483647LL;
+  return n >= 1 && n < 2147483647LL && m >= 1 && m <= (2147483647LL - LG_EDGE_CHUNK) / 2;
 }
 
 bool edge_args_ok(long long n, long long m, int dim, int dtype, long long ld) {

@@ -381,8 +381,8 @@ c10::intrusive_ptr<EdgeGraph> edge_graph(const Tensor& given, int64_t n) {
   TORCH_CHECK_VALUE(given.dim() == 2 && given.size(0) == 2, "idx must be (2, M), got shape ", given.sizes());
   auto g = c10::make_intrusive<EdgeGraph>();
   const int64_t m = given.size(1);
-  TORCH_CHECK_VALUE(n >= 1 && n <= kMaxRows && 2 * m <= kMaxRows,
-                    "n must be at least 1; at most 2^31 - 2 vertices and 2^30 - 1 edges");
+  TORCH_CHECK_VALUE(n >= 1 && n <= kMaxRows && m <= (2147483647 - LG_EDGE_CHUNK) / 2,
+                    "n must be at least 1; at most 2^31 - 2 vertices and 2^30 - 65 edges");
   g->n = n;
   g->m = m;
   g->device = given.device();

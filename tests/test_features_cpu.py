@@ -133,3 +133,12 @@ def test_edge_calls_refuse():
                 dict(nlong=1, nch=2, lr=P), dict(nlong=1, nch=2, lr=P, ws=P, nb=8)):
         assert grad(**bad) == BAD
     assert "lg_edge_sqdist_grad" in _native.last_error()
+
+
+def test_edge_lists_leave_room_in_32_bits():
+    """Positions a few beyond the last list entry, and a list's length rounded up to chunks of 128, fit an int."""
+    big, m = 1 << 62, (2 ** 31 - 1 - 128) // 2
+    assert L.lg_edge_graph_workspace_bytes(4, m) > 0 and L.lg_edge_graph_workspace_bytes(4, m + 1) == 0
+    assert L.lg_edge_graph(4, m + 1, P, P, P, P, P, P, P, big, None) == BAD
+    assert L.lg_edge_sqdist(4, m + 1, 3, 0, P, P, 3, P, P, big, None) == BAD
+    assert L.lg_edge_sqdist_grad(4, m + 1, 3, 0, P, P, P, 0, None, None, 0, None, None, P, 3, P, P, P, big, None) == BAD

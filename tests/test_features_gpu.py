@@ -879,3 +879,11 @@ def test_distances_drive_the_graph_gp():
     diff = (value(x + h * v) - value(x - h * v)) / (2 * h)
     # the difference's own error: h^2 of a smooth function's third derivative, and rounding 1e-12 / h
     assert abs(diff - float((gx * v).sum())) <= 1e-5 * max(1.0, abs(diff))
+
+
+def test_too_many_edges_are_refused():
+    from gpu_eigsh.features import EdgeDistances
+
+    idx = torch.zeros((2, 1), dtype=torch.int64, device="cuda").expand(2, 2 ** 30 - 64)   # a view: no memory
+    with pytest.raises(ValueError, match="edges"):
+        EdgeDistances(idx, 4)
