@@ -1,5 +1,5 @@
-// lg_feat.cuh — what the node-feature kernels (lg_rows.cu, lg_norm.cu,
-// lg_edges.cu) share: element types, vector accesses, the stable sort of row
+// lg_feat.cuh — what the node-feature kernels (lg_rows.cu, lg_norm_fwd.cu,
+// lg_norm_bwd.cu, lg_edges.cu) share: element types, vector accesses, the stable sort of row
 // ids, the column sum of partial rows.
 //
 // Element types are float, double, half and bfloat16.  Arithmetic and every

@@ -15,7 +15,7 @@
 // Lookup: one access per lane, the loads of four rows (short rows) or four
 // pieces of a row (long rows) in flight before the first store; short rows of an
 // awkward length lie in one line over the lanes.  Bound by memory: nothing is reused
-// but rows named twice.  10^6 x 64 fp32 by a permutation: 86 us, 5.9 TB/s.
+// but rows named twice.  10^6 x 64 fp32 by a permutation: 86 us, 6.0 TB/s.
 //
 // Gradient: the ids are sorted (stable, with their positions) and the sorted
 // positions cut into tiles of equal length; a group of lanes sums the rows of one
@@ -130,10 +130,10 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(GatherArgs a, const T*
 }
 
 // The vectors of all rows in one line, four a thread: for rows of up to 48 vectors
-// that would leave a sixth of the lanes above idle or more.  10^6 ids x 17 fp32: 32 us
-// instead of 59, 10^6 x 10 fp64 20 instead of 24, 606,060 x 33 fp32 38 instead of 60;
-// the division by the row length costs more where few lanes are idle (198,019 x 101
-// fp32: 37 instead of 24).
+// that would leave a sixth of the lanes above idle or more.  Of a table of 20,000 rows,
+// which L2 holds: 10^6 ids x 17 fp32: 32 us instead of 59, 10^6 x 10 fp64 20 instead of
+// 24, 606,060 x 33 fp32 38 instead of 60; the division by the row length costs more where
+// few lanes are idle (198,019 x 101 fp32: 37 instead of 24).
 template <typename T, int V, int MODE>
 __global__ void __launch_bounds__(kThreads) gather_flat_kernel(GatherArgs a, const T* __restrict__ table,
                                                                T* __restrict__ out) {
@@ -960,9 +960,10 @@ struct SumPlan {
 // long as they leave four blocks a SM.
 constexpr int kSms = 148;   // of a B200
 
-// Bytes cleared beside the sort: about what the SMs that do not sort write in its
-// time.  131072 x 2048 bf16 with 16384 ids: 122 us, 146 us with none, 130 us with all
-// 537 MB cleared there.
+// Bytes cleared beside the sort: about what the SMs that do not sort write in the time of
+// one of 16384 ids (23 us).  131072 x 2048 bf16 with 16384 ids: 122 us, 146 us with none,
+// 130 us with all 537 MB cleared there.  Sorts of fewer ids end before the clearing, those
+// of up to 131,072 (74 us) after it; what is not cleared here is by the sum's launch.
 constexpr long long kSideFillMost = 128LL << 20;
 
 SumPlan sum_plan(long long n, int nv, long long row_bytes) {
