@@ -95,6 +95,7 @@ def build_torch_binding(force: bool = False, verbose: bool = False) -> None:
         return
     if verbose:
         print(" ".join(cmd), flush=True)
+    TORCH_STAMP.unlink(missing_ok=True)   # a build that is cut short leaves none
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
