@@ -53,7 +53,7 @@ def _normalized(points) -> torch.Tensor:
     """Every point with mean 0 and variance 1 over its coordinates
     (gpu_eigsh.features.layer_norm in fp64), whatever the points' units: a point
     whose spread lies outside [1, 2^16) is first multiplied by the power of 2^16
-    that brings it there, which rounds nothing."""
+    that brings it there, which rounds nothing that its mean would keep."""
     from .features import layer_norm
 
     P = _device_points(points)
